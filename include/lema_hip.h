@@ -215,6 +215,17 @@ int lema_rmsnorm_bf16(const void* x, const void* d, const void* w, float eps, in
 int lema_cross_entropy_bf16(const void* logits, int64_t rows, int64_t V, int64_t ld,
                             const int64_t* target, float* loss, void* stream);
 
+/* lema_cross_entropy_bf16 that also keeps what the gradient needs: stats[r] = (max of the row,
+ * 1 / sum of e^(x - max)), two floats a row, for lema_token_logprobs_grad. stats may be NULL. */
+int lema_cross_entropy_stats_bf16(const void* logits, int64_t rows, int64_t V, int64_t ld,
+                                  const int64_t* target, float* loss, float* stats, void* stream);
+
+/* The gradients of out = silu(gate) * up: g_gate = gy up sig (1 + gate (1 - sig)) with
+ * sig = 1 / (1 + e^-gate), g_up = gy silu(gate); n bf16 elements as in lema_swiglu_bf16. The
+ * backward of SwiGLU.forward, code/lema/model.py:85-94. */
+int lema_swiglu_grad_bf16(const void* gate, const void* up, const void* gy, void* g_gate, void* g_up,
+                          int64_t n, void* stream);
+
 /* out[r * out_stride] = argmax of row r of bf16 values (V and the row stride ld multiples of
  * 8): the first index of the maximum, NaN above every number, as torch.argmax. Replaces the
  * greedy pick of code/lema/decode.py:71-93 (logits.argmax(-1)), written straight into a
@@ -226,6 +237,91 @@ int lema_argmax_bf16(const void* x, int64_t rows, int64_t V, int64_t ld, int64_t
  * the token embedding of a decode step (nn.Embedding, code/lema/model.py's tok_emb). */
 int lema_embedding_bf16(const void* table, int64_t vocab, int64_t D, const int64_t* ids,
                         int64_t n, void* out, void* stream);
+
+/* ---- a training step around the exact op: embedding, norms and losses with gradients ----
+ * All three value types. The reference trains these with torch's own operations
+ * (code/lema/model.py, code/lema/train.py); the policy and preference losses have no
+ * counterpart there. Work on the same workspace or outputs must be ordered by the caller. */
+
+/* out row i = table row ids[i] * scale, rounded once (the bits as they are where scale is 1),
+ * zeros for an id outside [0, vocab). table contiguous [vocab, D], 1 <= D <= 2^20, aligned to an
+ * element; rows of D % 8 == 0 on 16-byte boundaries are read in 16-byte pieces. */
+int lema_embedding(const void* table, int32_t dtype, int64_t vocab, int64_t D, const int64_t* ids,
+                   int64_t n, float scale, void* out, void* stream);
+
+/* The table's gradient: gw row v = scale * sum of gy row i over the positions i with ids[i] = v,
+ * summed in fp32 in a fixed order and rounded once; every row is written, zeros for tokens that
+ * do not occur and for token `padding` (negative: none). Ids outside [0, vocab) take no part.
+ *   gy   contiguous [n, D] of `dtype`; n < 2^31 - 16384, vocab and D at most 2^20
+ *   workspace  256-byte aligned, lema_embedding_grad_workspace_bytes(n, vocab, D) bytes: about
+ *              16 bytes a position, 4 a token, and n / 32 rows of fp32 */
+int64_t lema_embedding_grad_workspace_bytes(int64_t n, int64_t vocab, int64_t D);
+int lema_embedding_grad(const void* gy, int32_t dtype, const int64_t* ids, int64_t n, int64_t vocab,
+                        int64_t D, float scale, int64_t padding, void* gw, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
+/* Layer norm of s = x + d, the sum rounded to `dtype` and written to s_out (d NULL: s = x and
+ * s_out is unused): h_out = (s - mean) / sqrt(mean((s - mean)^2) + eps) * w + b in fp32, rounded
+ * once. w, b: [D], each may be NULL. rows < 2^31 contiguous rows of 1 <= D <= 16384. */
+int lema_layer_norm(const void* x, const void* d, const void* w, const void* b, int32_t dtype,
+                    float eps, int64_t rows, int64_t D, void* s_out, void* h_out, void* stream);
+
+/* The gradients of a norm of rows s: layer norm (center != 0) or RMS norm (center = 0, as
+ * lema_rmsnorm_bf16). With z the normalised row, r its factor and a = gh * w:
+ *   gx = gs + r (a - mean(a) [center only] - z mean(a z)), the gradient of s (and so of x and d);
+ *   gw = sum over rows of gh z,  gb = sum over rows of gh, in fp32 in a fixed order, rounded once.
+ * w and gs may be NULL (1 and 0), and any of gx, gw, gb that is not wanted (gb with center only).
+ *   workspace  256-byte aligned, lema_norm_grad_workspace_bytes(rows, D) bytes; NULL where
+ *              neither gw nor gb is wanted */
+int64_t lema_norm_grad_workspace_bytes(int64_t rows, int64_t D);
+int lema_norm_grad(const void* s, const void* w, const void* gh, const void* gs, int32_t dtype,
+                   int32_t center, float eps, int64_t rows, int64_t D, void* gx, void* gw, void* gb,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Log-probabilities of given tokens: lp[r] = log softmax(logits row r / temperature)[target[r]],
+ * NaN for a target outside [0, V).
+ *   logits  rows / inner by inner rows of V elements of `dtype`: row r starts at element
+ *           (r / inner) * so + (r % inner) * si; rows may start at any element
+ *   mask    NULL, or a byte a row: rows with 0 are not read and get lp 0
+ *   lp      fp32; lp64 NULL, or the same in 64 bits
+ *   stats   NULL, or two floats a row, (max, 1 / sum of e^((x - max) / temperature)), which the
+ *           gradient needs; nothing is written for rows that the mask leaves out */
+int lema_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t inner, int64_t V,
+                        int64_t so, int64_t si, const int64_t* target, const uint8_t* mask,
+                        float temperature, float* lp, double* lp64, float* stats, void* stream);
+
+/* The logits' gradient where each row's lp has the gradient c = coef[r / per] * *scale0 * *scale1
+ * (device scalars, NULL = 1): grad[r, j] = c / temperature * ([j = target[r]] - softmax[j]), in
+ * fp32, rounded once; grad contiguous [rows, V]. Rows with c = 0 and rows that the mask leaves
+ * out are not read: their gradient is zero. */
+int lema_token_logprobs_grad(const void* logits, int32_t dtype, int64_t rows, int64_t inner, int64_t V,
+                             int64_t so, int64_t si, const int64_t* target, const uint8_t* mask,
+                             float temperature, const float* stats, const float* coef, int64_t per,
+                             const float* scale0, const float* scale1, void* grad, void* stream);
+
+/* Clipped policy loss of sampled tokens, and what its gradient needs. Per row, with lp and stats as
+ * above, ratio = e^(lp - old_lp) and A = advantage:
+ *   term = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
+ *          + kl (e^(ref_lp - lp) - (ref_lp - lp) - 1)        (ref_lp NULL or kl 0: without)
+ *   coef = d term / d lp;  both 0 for rows that the mask leaves out
+ * loss = mean of the counted rows' terms (0 without any), inv_n = 1 / counted rows: the gradient
+ * of the loss is lema_token_logprobs_grad with coef, per = 1 and inv_n as a scale. */
+int lema_policy_loss(const void* logits, int32_t dtype, int64_t rows, int64_t inner, int64_t V,
+                     int64_t so, int64_t si, const int64_t* target, const uint8_t* mask,
+                     float temperature, const float* old_lp, const float* advantage,
+                     const float* ref_lp, float clip_low, float clip_high, float kl, float* lp,
+                     float* stats, float* term, float* coef, float* loss, float* inv_n, void* stream);
+
+/* Paired preference loss from token log-probabilities lp64 [2 * pairs, T], the chosen answers
+ * first, and the reference's ref_lp: with s the sum of an answer's counted lp64 - ref_lp,
+ *   margin = beta (s_chosen - s_rejected),
+ *   loss = mean of -(1 - label_smoothing) log sigmoid(margin)
+ *                  - label_smoothing log sigmoid(-margin),
+ *   coef[a] = d loss / d s of answer a, for lema_token_logprobs_grad with per = T.
+ * Sums in 64 bits. mask: NULL or a byte a token. pairs >= 1. */
+int lema_preference_loss(const double* lp64, const float* ref_lp, const uint8_t* mask, int64_t pairs,
+                         int64_t T, float beta, float label_smoothing, float* loss, float* margin,
+                         float* coef, void* stream);
 
 /* ---- decode-shaped products on the matrix cores (bf16, fp32 accumulation) ---- */
 

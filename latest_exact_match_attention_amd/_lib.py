@@ -27,6 +27,7 @@ FULL_MESSAGE = "hash table full: the store is presized and never grows -- provis
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
+_f32 = ctypes.c_float
 
 # name -> argument types, exactly the prototypes of include/lema_hip.h
 PROTOTYPES = {
@@ -59,6 +60,23 @@ PROTOTYPES = {
     "lema_argmax_bf16": ([_p, _i64, _i64, _i64, _p, _i64, _p], ctypes.c_int),
     "lema_embedding_bf16": ([_p, _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
     "lema_cross_entropy_bf16": ([_p, _i64, _i64, _i64, _p, _p, _p], ctypes.c_int),
+    "lema_cross_entropy_stats_bf16": ([_p, _i64, _i64, _i64, _p, _p, _p, _p], ctypes.c_int),
+    "lema_swiglu_grad_bf16": ([_p, _p, _p, _p, _p, _i64, _p], ctypes.c_int),
+    "lema_embedding": ([_p, _i32, _i64, _i64, _p, _i64, _f32, _p, _p], ctypes.c_int),
+    "lema_embedding_grad_workspace_bytes": ([_i64, _i64, _i64], ctypes.c_int64),
+    "lema_embedding_grad": ([_p, _i32, _p, _i64, _i64, _i64, _f32, _i64, _p, _p, _i64, _p],
+                            ctypes.c_int),
+    "lema_layer_norm": ([_p, _p, _p, _p, _i32, _f32, _i64, _i64, _p, _p, _p], ctypes.c_int),
+    "lema_norm_grad_workspace_bytes": ([_i64, _i64], ctypes.c_int64),
+    "lema_norm_grad": ([_p, _p, _p, _p, _i32, _i32, _f32, _i64, _i64, _p, _p, _p, _p, _i64, _p],
+                       ctypes.c_int),
+    "lema_token_logprobs": ([_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _f32, _p, _p, _p, _p],
+                            ctypes.c_int),
+    "lema_token_logprobs_grad": ([_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _f32, _p, _p, _i64,
+                                  _p, _p, _p, _p], ctypes.c_int),
+    "lema_policy_loss": ([_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _f32, _p, _p, _p, _f32, _f32,
+                          _f32, _p, _p, _p, _p, _p, _p, _p], ctypes.c_int),
+    "lema_preference_loss": ([_p, _p, _p, _i64, _i64, _f32, _f32, _p, _p, _p, _p], ctypes.c_int),
     "lema_skinny_gemm_bf16": ([_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _p], ctypes.c_int),
     "lema_skinny_pack_bf16": ([_p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _i64, _p, _i32, _p],
                               ctypes.c_int),
@@ -137,6 +155,37 @@ def stream_of(t: torch.Tensor) -> int:
     if _RAW_STREAM is None:
         return torch.cuda.current_stream(t.device).cuda_stream
     return _RAW_STREAM(t.get_device())
+
+
+class _Here:
+    """A `with` that changes nothing."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def device_of(t: torch.Tensor):
+    """Makes t's device the current one while a launch on its null stream is enqueued, which goes
+    to the current device."""
+    return _HERE if torch.cuda.current_device() == t.get_device() else torch.cuda.device(t.device)
+
+
+def same_device(t: torch.Tensor, **others) -> None:
+    """ValueError where a tensor (None is passed over) lies on another device than t."""
+    for name, o in others.items():
+        if o is not None and o.device != t.device:
+            raise ValueError(f"{name} is on {o.device}, expected {t.device}")
+
+
+def dense(t: torch.Tensor) -> torch.Tensor:
+    """t as the kernels read it: contiguous, its values the ones in memory."""
+    return t.resolve_neg().contiguous()
 
 
 # ---- host memory the GPU works on in place (a store table in host RAM) ----

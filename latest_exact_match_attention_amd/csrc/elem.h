@@ -1,0 +1,63 @@
+// Elements of the three value types as fp32: pieces of 16 bytes, and single elements.
+#pragma once
+#include "lema_internal.h"
+
+namespace lema {
+
+struct Bf16 {
+  uint16_t bits;
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(_Float16 v) { return static_cast<float>(v); }
+__device__ __forceinline__ float to_f32(Bf16 v) {
+  return __uint_as_float(static_cast<uint32_t>(v.bits) << 16);
+}
+
+// Round to nearest even; a NaN becomes the canonical quiet one in bf16.
+template <typename T>
+__device__ __forceinline__ T from_f32(float f);
+template <>
+__device__ __forceinline__ float from_f32<float>(float f) {
+  return f;
+}
+template <>
+__device__ __forceinline__ _Float16 from_f32<_Float16>(float f) {
+  return static_cast<_Float16>(f);
+}
+template <>
+__device__ __forceinline__ Bf16 from_f32<Bf16>(float f) {
+  const uint32_t b = __float_as_uint(f);
+  if ((b & 0x7F800000u) == 0x7F800000u && (b & 0x007FFFFFu) != 0) return Bf16{0x7FC0u};
+  return Bf16{static_cast<uint16_t>((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16)};
+}
+
+template <typename T>
+constexpr int kPiece = 16 / static_cast<int>(sizeof(T));  // elements of a 16-byte piece
+
+// A 16-byte piece as its elements.
+template <typename T>
+union Piece {
+  u32x4 raw;
+  T e[kPiece<T>];
+};
+
+// Calls f(T{}) with the element type of `dtype` (checked by the caller).
+template <typename F>
+inline void for_dtype(int32_t dtype, F f) {
+  if (dtype == LEMA_F32)
+    f(float{});
+  else if (dtype == LEMA_F16)
+    f(_Float16{});
+  else
+    f(Bf16{});
+}
+
+// Sum over the wavefront: every lane gets the same bits.
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+}  // namespace lema

@@ -1,0 +1,487 @@
+// Embedding lookup with a scale, and its gradient by sorted tokens.
+//
+// Forward: out row i = round(scale * table row ids[i]); a copy of the bits where scale is 1.
+//
+// Backward: gw row v = round(scale * sum of gy row i over the positions i with ids[i] = v), every row
+// of the table written, zeros where a token does not occur. Positions are first put in the order
+// of (token, position), which makes the sums' order fixed, without atomics on values:
+//   count    per span of positions, how many fall into each of up to 1024 buckets of tokens
+//            (the token's high bits);
+//   scatter  each span puts its positions, in order, into the buckets;
+//   order    each bucket orders its positions by token, and notes where each token's start;
+//   sum      a wavefront per (token, 512 columns) adds up to 64 rows. A longer list would
+//            keep one wavefront busy while the others end, so its whole tiles of 32 positions are
+//            summed by wavefronts of their own, in the same launch, in fp32;
+//   join     a workgroup per (long list, 512 columns) adds its tiles and its ragged ends.
+// A wavefront keeps its own cursors, so a place is a ballot per bit of the digit and needs no
+// atomics. gy is read once and the table's gradient written once, which bounds the work (HBM);
+// the ordering costs three short launches.
+#include "elem.h"
+
+namespace lema {
+namespace {
+
+constexpr int kBuckets = 1024;      // at most, of 1 << row_bits tokens each
+constexpr int kMaxRowBits = 10;     // so at most 2^20 tokens
+constexpr int kSpanStep = 1024;     // a span is a multiple of it: 16 wavefronts of 64
+constexpr int kTile = 32, kLong = 64;
+constexpr int kCols = 512;          // columns of a wavefront, 8 a lane
+
+__device__ __forceinline__ int wave_index() {
+  return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+}
+
+// A wavefront's row slice: 8 elements a lane from column c0 on, as fp32.
+template <typename T, bool kVec>
+__device__ __forceinline__ void load_slice(const T* row, int64_t c0, int64_t D, int lane, float (&v)[8]) {
+  if constexpr (kVec) {
+    constexpr int n = kPiece<T>;
+    const int64_t e = c0 + lane * 8;
+    Piece<T> q[8 / n];
+#pragma unroll
+    for (int i = 0; i < 8 / n; ++i)
+      q[i].raw = e < D ? *reinterpret_cast<const u32x4*>(row + e + i * n) : u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = to_f32(q[k / n].e[k % n]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t e = c0 + k * 64 + lane;
+      v[k] = e < D ? to_f32(row[e]) : 0.0f;
+    }
+  }
+}
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void store_slice(T* row, int64_t c0, int64_t D, int lane, const float (&v)[8]) {
+  if constexpr (kVec) {
+    constexpr int n = kPiece<T>;
+    const int64_t e = c0 + lane * 8;
+    if (e >= D) return;
+    Piece<T> q[8 / n];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) q[k / n].e[k % n] = from_f32<T>(v[k]);
+#pragma unroll
+    for (int i = 0; i < 8 / n; ++i) *reinterpret_cast<u32x4*>(row + e + i * n) = q[i].raw;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t e = c0 + k * 64 + lane;
+      if (e < D) row[e] = from_f32<T>(v[k]);
+    }
+  }
+}
+
+// One wavefront per (position, 512 columns).
+template <typename T, bool kVec, bool kScale>
+__global__ __launch_bounds__(256) void embed_kernel(const T* table, int64_t vocab, int64_t D,
+                                                    const int64_t* ids, int64_t n, int slices,
+                                                    float scale, T* out) {
+  const int lane = threadIdx.x & 63;
+  const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + wave_index();
+  const int64_t i = u / slices;
+  if (i >= n) return;
+  const int64_t c0 = (u - i * slices) * kCols, id = ids[i];
+  const bool ok = id >= 0 && id < vocab;
+  const T* src = table + (ok ? id : 0) * D;
+  T* dst = out + i * D;
+  if constexpr (kVec && !kScale) {  // the bits as they are
+    constexpr int p = kPiece<T>;
+    const int64_t e = c0 + lane * 8;
+    if (e >= D) return;
+#pragma unroll
+    for (int k = 0; k < 8 / p; ++k)
+      *reinterpret_cast<u32x4*>(dst + e + k * p) =
+          ok ? *reinterpret_cast<const u32x4*>(src + e + k * p) : u32x4{0, 0, 0, 0};
+  } else if constexpr (kVec) {
+    float v[8];
+    load_slice<T, true>(src, c0, D, lane, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = ok ? v[k] * scale : 0.0f;
+    store_slice<T, true>(dst, c0, D, lane, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t e = c0 + k * 64 + lane;
+      if (e < D) {
+        const T v = src[e];
+        dst[e] = ok ? (kScale ? from_f32<T>(to_f32(v) * scale) : v) : from_f32<T>(0.0f);
+      }
+    }
+  }
+}
+
+struct Order {            // what the ordering kernels share
+  const int64_t* ids;
+  int64_t n, vocab, padding;
+  int row_bits, buckets, spans;
+  int64_t span;
+  uint32_t* counts;       // [spans, kBuckets]
+  uint32_t* bucket_at;    // [kBuckets + 1]: where a bucket's positions start
+  uint32_t* item_pos;     // [n] positions by bucket
+  uint32_t* item_id;      // [n] their tokens
+  uint32_t* perm;         // [n] positions by (token, position)
+  uint32_t* token;        // [n] their tokens
+  uint32_t* start;        // [vocab + 1]
+  uint32_t* long_count;   // lists of more than kLong
+  uint32_t* long_list;    // their tokens, in no order
+};
+
+// Token of position i, or -1 for one that takes no part.
+__device__ __forceinline__ int64_t token_of(const Order& o, int64_t i, int64_t end) {
+  const int64_t id = i < end ? o.ids[i] : -1;
+  return id >= 0 && id < o.vocab && id != o.padding ? id : -1;
+}
+
+// Lanes whose `bits`-bit digit equals this lane's, among the lanes of `live`.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, uint64_t live) {
+  uint64_t m = live;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (digit >> b) & 1;
+    const uint64_t s = __ballot(one);
+    m &= one ? s : ~s;
+  }
+  return m;
+}
+
+// The place of each live lane's item from its digit's cursor, lanes in order; every lane of the
+// wavefront calls it.
+__device__ __forceinline__ uint32_t take_place(uint32_t* cursors, uint32_t digit, bool live, int bits,
+                                               int lane) {
+  const uint64_t m = same_digit(digit, bits, __ballot(live));
+  const uint32_t rank = __popcll(m & ((uint64_t(1) << lane) - 1));
+  uint32_t at = 0;
+  if (live) at = cursors[digit] + rank;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // every lane has read before one writes
+  if (live && rank == 0) cursors[digit] = at + __popcll(m);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  return at;
+}
+
+__global__ __launch_bounds__(1024) void embed_count_kernel(Order o) {
+  __shared__ uint32_t hist[kBuckets];
+  hist[threadIdx.x] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *o.long_count = 0;
+  __syncthreads();
+  const int64_t at = blockIdx.x * o.span, end = min(at + o.span, o.n);
+  for (int64_t i = at + threadIdx.x; i < end; i += 1024) {
+    const int64_t id = token_of(o, i, end);
+    if (id >= 0) atomicAdd(&hist[id >> o.row_bits], 1u);
+  }
+  __syncthreads();
+  o.counts[static_cast<int64_t>(blockIdx.x) * kBuckets + threadIdx.x] = hist[threadIdx.x];
+}
+
+// Exclusive sum over a workgroup's threads (kWaves wavefronts); `red` holds kWaves words.
+template <int kWaves>
+__device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* red) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  uint32_t s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t t = __shfl_up(s, d);
+    if (lane >= d) s += t;
+  }
+  if (lane == 63) red[w] = s;
+  __syncthreads();
+  uint32_t base = 0;
+  for (int i = 0; i < w; ++i) base += red[i];
+  return base + s - v;
+}
+
+// A span's positions into the buckets: 16 wavefronts on consecutive sixteenths of it.
+__global__ __launch_bounds__(1024) void embed_scatter_kernel(Order o) {
+  __shared__ uint32_t cur[16][kBuckets];
+  __shared__ uint32_t red[16];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int64_t part = o.span / 16;
+  const int64_t at = blockIdx.x * o.span + w * part;
+  const int64_t end = min(at + part, o.n);
+  for (int k = 0; k < 16; ++k) cur[k][t] = 0;
+  __syncthreads();
+  for (int64_t i = at + lane; i < end; i += 64) {
+    const int64_t id = token_of(o, i, end);
+    if (id >= 0) atomicAdd(&cur[w][id >> o.row_bits], 1u);
+  }
+  // thread t: bucket t's positions in all spans, and in the spans before this one
+  uint32_t all = 0, before = 0;
+#pragma unroll 8
+  for (int s = 0; s < o.spans; ++s) {
+    const uint32_t c = o.counts[static_cast<int64_t>(s) * kBuckets + t];
+    all += c;
+    before += s < static_cast<int>(blockIdx.x) ? c : 0u;
+  }
+  uint32_t base = group_scan<16>(all, red);  // its barrier also ends the counting above
+  if (blockIdx.x == 0) {
+    o.bucket_at[t] = base;
+    if (t == kBuckets - 1) o.bucket_at[kBuckets] = base + all;
+  }
+  base += before;
+  for (int k = 0; k < 16; ++k) {
+    const uint32_t c = cur[k][t];
+    cur[k][t] = base;
+    base += c;
+  }
+  __syncthreads();
+  for (int64_t i0 = at; i0 < end; i0 += 64) {
+    const int64_t id = token_of(o, i0 + lane, end);
+    const uint32_t place =
+        take_place(cur[w], static_cast<uint32_t>((id < 0 ? 0 : id) >> o.row_bits), id >= 0, 10, lane);
+    if (id >= 0) {
+      o.item_pos[place] = static_cast<uint32_t>(i0 + lane);
+      o.item_id[place] = static_cast<uint32_t>(id);
+    }
+  }
+}
+
+// One workgroup per bucket: its positions ordered by token, and where each token's start.
+__global__ __launch_bounds__(512) void embed_order_kernel(Order o) {
+  __shared__ uint32_t cur[8][1 << kMaxRowBits];
+  __shared__ uint32_t red[8];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int rows = 1 << o.row_bits;
+  const uint32_t b0 = o.bucket_at[blockIdx.x], b1 = o.bucket_at[blockIdx.x + 1];
+  const uint32_t part = ((b1 - b0) / 512 + 1) * 64;  // 8 parts cover the bucket
+  const uint32_t at = min(b0 + w * part, b1), end = min(at + part, b1);
+  for (int k = t; k < 8 * rows; k += 512) cur[k / rows][k % rows] = 0;
+  __syncthreads();
+  for (uint32_t i = at + lane; i < end; i += 64) atomicAdd(&cur[w][o.item_id[i] & (rows - 1)], 1u);
+  __syncthreads();
+  uint32_t mine[2] = {0, 0};  // tokens 2 t and 2 t + 1 of the bucket
+  for (int j = 0; j < 2; ++j)
+    if (2 * t + j < rows)
+      for (int k = 0; k < 8; ++k) mine[j] += cur[k][2 * t + j];
+  uint32_t base = b0 + group_scan<8>(mine[0] + mine[1], red);
+  for (int j = 0; j < 2; ++j) {
+    const int r = 2 * t + j;
+    const int64_t v = (static_cast<int64_t>(blockIdx.x) << o.row_bits) + r;
+    if (r < rows) {
+      if (v < o.vocab) {
+        o.start[v] = base;
+        if (v == o.vocab - 1) o.start[o.vocab] = b1;
+        if (mine[j] > kLong) o.long_list[atomicAdd(o.long_count, 1u)] = static_cast<uint32_t>(v);
+      }
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t c = cur[k][r];
+        cur[k][r] = base;
+        base += c;
+      }
+    }
+  }
+  __syncthreads();
+  for (uint32_t i0 = at; i0 < end; i0 += 64) {
+    const bool live = i0 + lane < end;
+    const uint32_t id = live ? o.item_id[i0 + lane] : 0u;
+    const uint32_t place = take_place(cur[w], id & (rows - 1), live, o.row_bits, lane);
+    if (live) {
+      o.perm[place] = o.item_pos[i0 + lane];
+      o.token[place] = id;
+    }
+  }
+}
+
+// acc += gy rows perm[j], j in [j0, j1), in order: 64 positions read at once, 4 rows in flight.
+template <typename T, bool kVec>
+__device__ __forceinline__ void add_rows(const T* gy, const uint32_t* perm, uint32_t j0, uint32_t j1,
+                                         int64_t c0, int64_t D, int lane, float (&acc)[8]) {
+  for (uint32_t j = j0; j < j1; j += 64) {
+    const int m = min(64u, j1 - j);
+    const uint32_t pos = perm[j + min(lane, m - 1)];
+    for (int i = 0; i < m; i += 4) {
+      float v[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t p = __builtin_amdgcn_readlane(pos, min(i + u, m - 1));
+        load_slice<T, kVec>(gy + static_cast<int64_t>(p) * D, c0, D, lane, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += i + u < m ? v[u][k] : 0.0f;
+    }
+  }
+}
+
+// One wavefront per (tile or token, 512 columns): the tiles come first. partial: [tiles, D].
+template <typename T, bool kVec>
+__global__ __launch_bounds__(256) void embed_sum_kernel(Order o, const T* gy, int64_t D, int slices,
+                                                        int64_t tiles, float scale, float* partial,
+                                                        T* gw) {
+  const int lane = threadIdx.x & 63;
+  const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + wave_index();
+  const int64_t item = u / slices, c0 = (u - item * slices) * kCols;
+  if (item >= tiles + o.vocab) return;
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (item < tiles) {
+    const uint32_t j0 = static_cast<uint32_t>(item) * kTile;
+    if (j0 + kTile > o.start[o.vocab]) return;
+    const uint32_t v = o.token[j0];
+    if (o.token[j0 + kTile - 1] != v || o.start[v + 1] - o.start[v] <= kLong) return;
+    add_rows<T, kVec>(gy, o.perm, j0, j0 + kTile, c0, D, lane, acc);
+    store_slice<float, kVec>(partial + item * D, c0, D, lane, acc);
+  } else {
+    const int64_t v = item - tiles;
+    const uint32_t j0 = o.start[v], j1 = o.start[v + 1];
+    if (j1 - j0 > kLong) return;
+    add_rows<T, kVec>(gy, o.perm, j0, j1, c0, D, lane, acc);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] *= scale;
+    store_slice<T, kVec>(gw + v * D, c0, D, lane, acc);
+  }
+}
+
+// One workgroup per (long list, 512 columns). A list of more than 64 holds a whole tile at least.
+template <typename T, bool kVec>
+__global__ __launch_bounds__(256) void embed_join_kernel(Order o, const T* gy, int64_t D, float scale,
+                                                         const float* partial, T* gw) {
+  __shared__ float sums[4][8][64];
+  if (blockIdx.x >= *o.long_count) return;
+  const int lane = threadIdx.x & 63, w = wave_index();
+  const int64_t v = o.long_list[blockIdx.x], c0 = static_cast<int64_t>(blockIdx.y) * kCols;
+  const uint32_t j0 = o.start[v], j1 = o.start[v + 1];
+  const uint32_t t0 = (j0 + kTile - 1) / kTile, t1 = j1 / kTile;
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (w == 0) add_rows<T, kVec>(gy, o.perm, j0, t0 * kTile, c0, D, lane, acc);
+  if (w == 1) add_rows<T, kVec>(gy, o.perm, t1 * kTile, j1, c0, D, lane, acc);
+  for (uint32_t t = t0 + w; t < t1; t += 4) {
+    float p[8];
+    load_slice<float, kVec>(partial + static_cast<int64_t>(t) * D, c0, D, lane, p);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] += p[k];
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sums[w][k][lane] = acc[k];
+  __syncthreads();
+  if (w != 0) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    acc[k] = (acc[k] + sums[1][k][lane] + sums[2][k][lane] + sums[3][k][lane]) * scale;
+  store_slice<T, kVec>(gw + v * D, c0, D, lane, acc);
+}
+
+int64_t span_of(int64_t n) {
+  // about 64 spans, of 1024 to 16384 positions
+  const int64_t s = (n / 64 + kSpanStep - 1) / kSpanStep * kSpanStep;
+  return s < kSpanStep ? kSpanStep : s > 16 * kSpanStep ? 16 * kSpanStep : s;
+}
+
+// Fills `o` and the address of the tiles' sums for a workspace at `ws`; returns its bytes.
+int64_t lay_out(Order& o, float*& partial, void* ws, int64_t n, int64_t vocab, int64_t D) {
+  o.n = n;
+  o.vocab = vocab;
+  o.row_bits = 0;
+  while (((vocab - 1) >> o.row_bits) >= kBuckets) ++o.row_bits;
+  o.buckets = static_cast<int>((vocab - 1) >> o.row_bits) + 1;
+  o.span = span_of(n);
+  o.spans = static_cast<int>((n + o.span - 1) / o.span);
+  if (o.spans < 1) o.spans = 1;
+  char* base = static_cast<char*>(ws);
+  int64_t used = 0;
+  const auto take = [&](int64_t count) {
+    const int64_t at = used;
+    used += (count * 4 + 255) / 256 * 256;
+    return base == nullptr ? nullptr : base + at;
+  };
+  const auto words = [&](int64_t count) { return reinterpret_cast<uint32_t*>(take(count)); };
+  o.counts = words(static_cast<int64_t>(o.spans) * kBuckets);
+  o.bucket_at = words(kBuckets + 1);
+  o.item_pos = words(n);
+  o.item_id = words(n);
+  o.perm = words(n);
+  o.token = words(n);
+  o.start = words(vocab + 1);
+  o.long_count = words(1);
+  o.long_list = words(n / kLong + 1);
+  partial = reinterpret_cast<float*>(take(n / kTile * D));
+  return used;
+}
+
+bool sizes_ok(int64_t n, int64_t vocab, int64_t D) {
+  return n >= 0 && n < (int64_t(1) << 31) - 16 * kSpanStep && vocab >= 1 &&
+         vocab <= int64_t(kBuckets) << kMaxRowBits && D >= 1 && D <= (int64_t(1) << 20);
+}
+
+}  // namespace
+
+int embed_launch(const void* table, int32_t dtype, int64_t vocab, int64_t D, const int64_t* ids,
+                 int64_t n, float scale, void* out, hipStream_t st) {
+  const int64_t slices = (D + kCols - 1) / kCols;
+  const int64_t grid = (n * slices + 3) / 4;
+  LEMA_REQUIRE(grid < (int64_t(1) << 31), "too many ids");
+  const bool vec = D % 8 == 0 && aligned(table, 16) && aligned(out, 16), scaled = scale != 1.0f;
+  for_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    const auto kernel = vec ? (scaled ? embed_kernel<T, true, true> : embed_kernel<T, true, false>)
+                            : (scaled ? embed_kernel<T, false, true> : embed_kernel<T, false, false>);
+    kernel<<<dim3(grid), dim3(256), 0, st>>>(static_cast<const T*>(table), vocab, D, ids, n,
+                                             static_cast<int>(slices), scale, static_cast<T*>(out));
+  });
+  return launch_status("embed_kernel");
+}
+
+}  // namespace lema
+
+using namespace lema;
+
+extern "C" int lema_embedding(const void* table, int32_t dtype, int64_t vocab, int64_t D,
+                              const int64_t* ids, int64_t n, float scale, void* out, void* stream) {
+  clear_error();
+  const int size = dtype_size(dtype);
+  LEMA_REQUIRE(size != 0, "unknown dtype %d", dtype);
+  LEMA_REQUIRE(vocab >= 1 && D >= 1 && D <= (int64_t(1) << 20) && n >= 0 && n < (int64_t(1) << 31),
+               "bad sizes: %lld ids, table [%lld, %lld]", (long long)n, (long long)vocab, (long long)D);
+  if (n == 0) return LEMA_OK;
+  LEMA_REQUIRE(table && ids && out && aligned(table, size) && aligned(ids, 8) && aligned(out, size),
+               "bad pointer");
+  return embed_launch(table, dtype, vocab, D, ids, n, scale, out, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int64_t lema_embedding_grad_workspace_bytes(int64_t n, int64_t vocab, int64_t D) {
+  if (!sizes_ok(n, vocab, D)) return 0;
+  Order o;
+  float* partial;
+  return lay_out(o, partial, nullptr, n, vocab, D);
+}
+
+extern "C" int lema_embedding_grad(const void* gy, int32_t dtype, const int64_t* ids, int64_t n,
+                                   int64_t vocab, int64_t D, float scale, int64_t padding, void* gw,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  const int size = dtype_size(dtype);
+  LEMA_REQUIRE(size != 0, "unknown dtype %d", dtype);
+  LEMA_REQUIRE(sizes_ok(n, vocab, D),
+               "bad sizes: %lld ids, table [%lld, %lld] (at most 2^20 tokens and columns)", (long long)n,
+               (long long)vocab, (long long)D);
+  LEMA_REQUIRE(gw && aligned(gw, size) && (n == 0 || (gy && ids && aligned(gy, size) && aligned(ids, 8))),
+               "bad pointer");
+  LEMA_REQUIRE(workspace && aligned(workspace, 256) &&
+                   workspace_bytes >= lema_embedding_grad_workspace_bytes(n, vocab, D),
+               "the gradient needs a workspace of %lld bytes",
+               (long long)lema_embedding_grad_workspace_bytes(n, vocab, D));
+  Order o;
+  float* partial;
+  lay_out(o, partial, workspace, n, vocab, D);
+  o.ids = ids;
+  o.padding = padding;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t slices = (D + kCols - 1) / kCols, tiles = n / kTile, longest = n / (kLong + 1);
+  const int64_t grid = ((tiles + vocab) * slices + 3) / 4;
+  LEMA_REQUIRE(grid < (int64_t(1) << 31), "table [%lld, %lld] is too large", (long long)vocab,
+               (long long)D);
+  embed_count_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
+  embed_scatter_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
+  embed_order_kernel<<<dim3(o.buckets), dim3(512), 0, st>>>(o);
+  const bool vec = D % 8 == 0 && aligned(gy, 16) && aligned(gw, 16);
+  for_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    const auto sum = vec ? embed_sum_kernel<T, true> : embed_sum_kernel<T, false>;
+    sum<<<dim3(grid), dim3(256), 0, st>>>(o, static_cast<const T*>(gy), D, static_cast<int>(slices),
+                                          tiles, scale, partial, static_cast<T*>(gw));
+    if (longest > 0) {
+      const auto join = vec ? embed_join_kernel<T, true> : embed_join_kernel<T, false>;
+      join<<<dim3(longest, slices), dim3(256), 0, st>>>(o, static_cast<const T*>(gy), D, scale, partial,
+                                                        static_cast<T*>(gw));
+    }
+  });
+  return launch_status("the embedding gradient's kernels");
+}

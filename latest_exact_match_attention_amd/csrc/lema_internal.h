@@ -6,6 +6,8 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
+#include <type_traits>
 
 #include "../../include/lema_hip.h"
 
@@ -73,6 +75,10 @@ struct FastDiv {
 int pack_launch(const void* z, void* codes, const void* z2, void* codes2, int32_t dtype, int64_t B, int64_t H,
                 int64_t T, int32_t D, int64_t z_sb, int64_t z_sh, int64_t z_st, int32_t code_bytes,
                 hipStream_t st);
+
+// embed.hip: out row i = scale * table row ids[i] (arguments checked, n > 0).
+int embed_launch(const void* table, int32_t dtype, int64_t vocab, int64_t D, const int64_t* ids,
+                 int64_t n, float scale, void* out, hipStream_t st);
 
 // MI355X dispatches consecutive workgroups round-robin over its 8 XCDs, each with its own
 // 4 MB L2; kernels map blockIdx so that work sharing data lands on one XCD.

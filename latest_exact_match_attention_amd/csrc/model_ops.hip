@@ -9,7 +9,9 @@
 //               of the row (online max and rescaled sum), instead of a fp32 copy plus a
 //               softmax pass;
 //   argmax      a decode step's greedy pick, written straight into the token buffer;
-//   embedding   the token embedding rows of a decode step, one workgroup per row.
+//   embedding   the token embedding rows of a decode step (kernel in embed.hip);
+// and the gradient of swiglu, for training through the MLP. The loss keeps (max, 1 / sum) of a
+// row where its gradient is wanted (loss.hip).
 #include "lema_internal.h"
 #include "norm_row.h"
 
@@ -61,6 +63,34 @@ __global__ __launch_bounds__(256) void swiglu_kernel(const u32x4* gate, const u3
   }
 }
 
+// y = s u with s = g sig, sig = 1 / (1 + e^-g):  gu = gy s,  gg = gy u sig (1 + g (1 - sig)), in
+// fp32 with one rounding each; a piece of each input per thread and trip.
+__global__ __launch_bounds__(256) void swiglu_grad_kernel(const u32x4* gate, const u32x4* up,
+                                                          const u32x4* gy, u32x4* g_gate, u32x4* g_up,
+                                                          int64_t n8) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n8; i += stride) {
+    const u32x4 gv = gate[i], uv = up[i], yv = gy[i];
+    u32x4 og, ou;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t a = 0, b = 0;
+#pragma unroll
+      for (int h = 0; h < 32; h += 16) {
+        const float g = bf16_to_f32((gv[k] >> h) & 0xFFFFu), u = bf16_to_f32((uv[k] >> h) & 0xFFFFu);
+        const float y = bf16_to_f32((yv[k] >> h) & 0xFFFFu);
+        const float sig = 1.0f / (1.0f + expf(-g));
+        a |= f32_to_bf16(y * u * sig * (1.0f + g * (1.0f - sig))) << h;
+        b |= f32_to_bf16(y * (g * sig)) << h;
+      }
+      og[k] = a;
+      ou[k] = b;
+    }
+    g_gate[i] = og;
+    g_up[i] = ou;
+  }
+}
+
 // One wavefront per row of D bf16 (D % 8 == 0, D <= 512 * S).
 template <int S>
 __global__ __launch_bounds__(256) void rmsnorm_kernel(const uint16_t* x, const uint16_t* d,
@@ -88,7 +118,8 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const uint16_t* x, const u
 // trip the kernel was bound by VALU issue: 4096 x 50304 logits took 114-133 us, now 75 us
 // (5.4 TB/s), at the same error against an fp32 cross-entropy (about 2e-7 per row).
 __global__ __launch_bounds__(256) void xent_kernel(const uint16_t* logits, int64_t V, int64_t ld,
-                                                   const int64_t* target, float* loss) {
+                                                   const int64_t* target, float* loss,
+                                                   float2* stats) {
   __shared__ float smax[4], ssum[4];
   constexpr float kLog2e = 1.4426950408889634f;
   const int64_t row = blockIdx.x;
@@ -146,6 +177,7 @@ __global__ __launch_bounds__(256) void xent_kernel(const uint16_t* logits, int64
     const int64_t t = target[row];
     const float xt = (t >= 0 && t < V) ? bf16_to_f32(r[t]) : NAN;
     loss[row] = logf(S) + M - xt;
+    if (stats != nullptr) stats[row] = make_float2(M, 1.0f / S);
   }
 }
 
@@ -167,6 +199,22 @@ extern "C" int lema_swiglu_bf16(const void* gate, const void* up, void* out, int
   swiglu_kernel<<<dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
       static_cast<const u32x4*>(gate), static_cast<const u32x4*>(up), static_cast<u32x4*>(out), n8);
   return launch_status("swiglu_kernel");
+}
+
+extern "C" int lema_swiglu_grad_bf16(const void* gate, const void* up, const void* gy, void* g_gate,
+                                     void* g_up, int64_t n, void* stream) {
+  clear_error();
+  LEMA_REQUIRE(n >= 0 && n % 8 == 0, "element count %lld must be a multiple of 8", (long long)n);
+  if (n == 0) return LEMA_OK;
+  for (const void* p : {gate, up, gy, static_cast<const void*>(g_gate), static_cast<const void*>(g_up)})
+    LEMA_REQUIRE(p && aligned(p, 16), "all five must be 16-byte aligned device pointers");
+  const int64_t n8 = n / 8;
+  int64_t grid = (n8 + 255) / 256;
+  if (grid > 65536) grid = 65536;
+  swiglu_grad_kernel<<<dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+      static_cast<const u32x4*>(gate), static_cast<const u32x4*>(up), static_cast<const u32x4*>(gy),
+      static_cast<u32x4*>(g_gate), static_cast<u32x4*>(g_up), n8);
+  return launch_status("swiglu_grad_kernel");
 }
 
 extern "C" int lema_rmsnorm_bf16(const void* x, const void* d, const void* w, float eps,
@@ -251,33 +299,25 @@ __global__ __launch_bounds__(1024) void argmax_kernel(const uint16_t* x, int64_t
   }
 }
 
-// One workgroup per id: out row i = table row ids[i] (D bf16, D % 8 == 0, 16-byte aligned
-// rows), or zeros for an id outside [0, vocab).
-__global__ __launch_bounds__(256) void embedding_kernel(const uint16_t* table, int64_t vocab,
-                                                        int64_t D, const int64_t* ids,
-                                                        uint16_t* out) {
-  const int64_t i = blockIdx.x;
-  const int64_t id = ids[i];
-  const bool ok = id >= 0 && id < vocab;
-  const u32x4* src = reinterpret_cast<const u32x4*>(table + (ok ? id : 0) * D);
-  u32x4* dst = reinterpret_cast<u32x4*>(out + i * D);
-  for (int64_t k = threadIdx.x; k < D / 8; k += blockDim.x)
-    dst[k] = ok ? src[k] : u32x4{0u, 0u, 0u, 0u};
-}
-
-extern "C" int lema_cross_entropy_bf16(const void* logits, int64_t rows, int64_t V, int64_t ld,
-                                       const int64_t* target, float* loss, void* stream) {
+extern "C" int lema_cross_entropy_stats_bf16(const void* logits, int64_t rows, int64_t V, int64_t ld,
+                                             const int64_t* target, float* loss, float* stats,
+                                             void* stream) {
   clear_error();
   LEMA_REQUIRE(rows >= 0 && V > 0 && V % 8 == 0 && ld >= V && ld % 8 == 0,
                "vocabulary %lld and row stride %lld must be multiples of 8", (long long)V,
                (long long)ld);
   if (rows == 0) return LEMA_OK;
   LEMA_REQUIRE(logits && target && loss && aligned(logits, 16) && aligned(target, 8) &&
-                   aligned(loss, 4), "bad pointer");
+                   aligned(loss, 4) && aligned(stats, 8), "bad pointer");
   LEMA_REQUIRE(rows < (int64_t(1) << 31), "too many rows");
   xent_kernel<<<dim3(rows), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(logits), V, ld, target, loss);
+      static_cast<const uint16_t*>(logits), V, ld, target, loss, reinterpret_cast<float2*>(stats));
   return launch_status("xent_kernel");
+}
+
+extern "C" int lema_cross_entropy_bf16(const void* logits, int64_t rows, int64_t V, int64_t ld,
+                                       const int64_t* target, float* loss, void* stream) {
+  return lema_cross_entropy_stats_bf16(logits, rows, V, ld, target, loss, nullptr, stream);
 }
 
 extern "C" int lema_argmax_bf16(const void* x, int64_t rows, int64_t V, int64_t ld, int64_t* out,
@@ -307,7 +347,5 @@ extern "C" int lema_embedding_bf16(const void* table, int64_t vocab, int64_t D, 
   LEMA_REQUIRE(n > 0 && n < (int64_t(1) << 31), "bad id count %lld", (long long)n);
   LEMA_REQUIRE(table && ids && out && aligned(table, 16) && aligned(ids, 8) && aligned(out, 16),
                "bad pointer");
-  embedding_kernel<<<dim3(n), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(table), vocab, D, ids, static_cast<uint16_t*>(out));
-  return launch_status("embedding_kernel");
+  return embed_launch(table, LEMA_BF16, vocab, D, ids, n, 1.0f, out, static_cast<hipStream_t>(stream));
 }

@@ -79,6 +79,7 @@ class LemaDecoder:
         segs = [b.seg or (b.gpu_pre, b.gpu_post) for b in model.blocks]
         choose = _chooser(temperature)
 
+        @torch.no_grad()
         def step_fn():
             x = embed(model.tok_emb, self.tok)
             for i in range(L):

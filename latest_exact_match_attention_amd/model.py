@@ -14,6 +14,9 @@ block norm1, q, k, v, o, norm2, gate, up, down, then norm_f, lm_head; Gaussian s
 outputs scaled by 1/sqrt(2 * depth): code/lema/model.py:258-281), so the same seed gives the
 same weights.
 
+Forwards without a cache are differentiable where the exact op is (in the values, not in the
+codes): the embedding, the norms, SwiGLU and the loss have hand-written gradients in bf16.
+
 In bf16 on the GPU the SwiGLU product, both pre-norms (the MLP's with the attention residual
 add), the final norm and the loss run as fused HIP kernels (the reference compiles these
 segments with torch.compile). The norm kernel rounds like torch's RMSNorm (one rounding of
@@ -29,6 +32,7 @@ exact-match path.
 """
 from __future__ import annotations
 
+import contextlib
 import dataclasses
 import math
 from dataclasses import dataclass
@@ -37,12 +41,13 @@ from pathlib import Path
 import torch
 import torch.nn.functional as F
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .attention import code_dtype_for, lema_from_codes, lema_hard, pack_codes
 
 __all__ = ["ModelConfig", "SwiGLU", "Attention", "Block", "Transformer", "lm_loss", "rms_norm",
-           "embed", "argmax_into", "load_trained",
+           "layer_norm", "embed", "argmax_into", "load_trained",
            "swiglu", "cross_entropy_sum"]
 
 # ------------------------------------------------------------------ fused bf16 segments
@@ -56,36 +61,182 @@ def _fused(*ts: torch.Tensor) -> bool:
     return True
 
 
+def _needs_grad(*ts) -> bool:
+    """Whether autograd wants a gradient of one of the tensors (None is passed over)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _saved(t: torch.Tensor, like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A saved tensor as it was saved: a saved-tensor hook may bring it back in another form."""
+    return _lib.dense(t.to(device=like.device, dtype=dtype))
+
+
+def _norm_forward(x, d, w, b, eps, center):
+    """h and s = x + d (None without d) of contiguous inputs, w's elements to a row."""
+    D = w.numel() if isinstance(w, torch.Tensor) else w
+    w = w if isinstance(w, torch.Tensor) else None
+    h = torch.empty_like(x)
+    s = torch.empty_like(x) if d is not None else None
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    with _lib.device_of(x):
+        if center:
+            _lib.check(_lib.lib().lema_layer_norm(
+                x.data_ptr(), ptr(d), ptr(w), ptr(b), _lib.DTYPE_CODE[x.dtype], eps, x.numel() // D, D,
+                ptr(s), h.data_ptr(), _lib.stream_of(x)))
+        else:
+            _lib.check(_lib.lib().lema_rmsnorm_bf16(
+                x.data_ptr(), ptr(d), ptr(w), eps, x.numel() // D, D, ptr(s), h.data_ptr(),
+                _lib.stream_of(x)))
+    return h, s
+
+
+class _Norm(torch.autograd.Function):
+    """h, and s = x + d where d is given, with the gradients of x, d and the weights."""
+
+    @staticmethod
+    def forward(ctx, x, d, w, b, D, eps, center):
+        h, s = _norm_forward(x, d, w if w is not None else D, b, eps, center)
+        ctx.save_for_backward(x if s is None else s, w)
+        ctx.norm = D, eps, center, d is not None, b is not None
+        ctx.w_shape = w.shape if w is not None else b.shape if b is not None else None
+        ctx.set_materialize_grads(False)
+        return h if s is None else (h, s)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gh, gs=None):
+        D, eps, center, has_d, has_b = ctx.norm
+        want_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        want_w, want_b = ctx.needs_input_grad[2:4]
+        if gh is None:                                # only the sum was used
+            return gs, gs, None, None, None, None, None
+        s, w = ctx.saved_tensors
+        gh = _lib.dense(gh)
+        gs = _lib.dense(gs) if gs is not None else None
+        s = _saved(s, gh, gh.dtype)
+        w = _saved(w, gh, gh.dtype) if w is not None else None
+        rows = s.numel() // D
+        gx = torch.empty_like(s) if want_x else None
+        gw = gh.new_empty(D) if want_w else None
+        gb = gh.new_empty(D) if want_b and has_b else None
+        L = _lib.lib()
+        n = L.lema_norm_grad_workspace_bytes(rows, D) if want_w or want_b else 0
+        ws = gh.new_empty(n, dtype=torch.uint8)
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        with _lib.device_of(gh):
+            _lib.check(L.lema_norm_grad(
+                s.data_ptr(), ptr(w), gh.data_ptr(), ptr(gs), _lib.DTYPE_CODE[s.dtype], int(center), eps,
+                rows, D, ptr(gx), ptr(gw), ptr(gb), ws.data_ptr() if n else None, n, _lib.stream_of(gh)))
+        shape = lambda g: g.view(ctx.w_shape) if g is not None else None  # noqa: E731
+        return gx, gx if has_d else None, shape(gw), shape(gb), None, None, None
+
+
 def rms_norm(x: torch.Tensor, norm: nn.RMSNorm, d: torch.Tensor | None = None):
-    """norm(x + d) and x + d (or norm(x), x when d is None), one pass in bf16."""
+    """norm(x + d) and x + d (or norm(x), x when d is None), one pass in bf16; the gradients of
+    x, d and the weight take one more and a sum over workgroups."""
     if d is not None and not (_fused(x, d) and _fused(norm.weight)):
         x, d = x + d, None
     if not (_fused(x) and _fused(norm.weight) and x.shape[-1] % 8 == 0
             and x.shape[-1] <= 4096):
         return norm(x), x
-    D = x.shape[-1]
-    h = torch.empty_like(x)
-    xo = torch.empty_like(x) if d is not None else x
-    eps = norm.eps if norm.eps is not None else torch.finfo(x.dtype).eps
-    _lib.check(_lib.lib().lema_rmsnorm_bf16(
-        x.data_ptr(), d.data_ptr() if d is not None else None, norm.weight.data_ptr(),
-        float(eps), x.numel() // D, D, xo.data_ptr() if d is not None else None, h.data_ptr(),
-        _lib.stream_of(x)))
-    return h, xo
+    eps = float(norm.eps if norm.eps is not None else torch.finfo(x.dtype).eps)
+    return _norm(x, d, norm.weight, None, x.shape[-1], eps, False)
 
 
-def embed(emb: nn.Embedding, ids: torch.Tensor) -> torch.Tensor:
-    """emb(ids) for a decode step: bf16 rows gathered by one workgroup each. The ids must lie
-    in [0, vocab) (an id outside it gives a zero row where nn.Embedding raises)."""
-    w = emb.weight
-    if not (_fused(w) and ids.is_cuda and ids.dtype == torch.long and ids.is_contiguous()
-            and w.shape[1] % 8 == 0 and w.data_ptr() % 16 == 0):
-        return emb(ids)
-    out = torch.empty(ids.shape + (w.shape[1],), dtype=w.dtype, device=w.device)
-    _lib.check(_lib.lib().lema_embedding_bf16(w.data_ptr(), w.shape[0], w.shape[1],
-                                              ids.data_ptr(), ids.numel(), out.data_ptr(),
-                                              _lib.stream_of(w)))
+def _norm(x, d, w, b, D, eps, center):
+    if _needs_grad(x, d, w, b):
+        out = _Norm.apply(x, d, w, b, D, eps, center)
+        return out if d is not None else (out, x)
+    h, s = _norm_forward(x, d, w if w is not None else D, b, eps, center)
+    return h, s if d is not None else x
+
+
+LAYER_NORM_MAX = 16384  # elements of a row that the kernels hold in registers
+
+
+def layer_norm(x: torch.Tensor, norm: nn.LayerNorm, d: torch.Tensor | None = None):
+    """norm(x + d) and x + d (or norm(x), x when d is None), as rms_norm for an nn.LayerNorm: one
+    pass on the GPU in float32, float16 or bfloat16, the sum rounded to that type first, mean and
+    variance in fp32 from the centred row. Differentiable in x, d, weight and bias. Rows of at
+    most 16384 elements of any length and alignment; the parameters have x's type. On the CPU, and
+    in float64, the torch operations."""
+    if d is not None and d.shape != x.shape:
+        raise ValueError(f"the addend {tuple(d.shape)} does not match x {tuple(x.shape)}")
+    if not x.is_cuda or x.dtype not in _lib.DTYPE_CODE:
+        x = x if d is None else x + d
+        return norm(x), x
+    dims = tuple(norm.normalized_shape)
+    if tuple(x.shape[x.dim() - len(dims):]) != dims:
+        raise ValueError(f"x {tuple(x.shape)} does not end in the norm's shape {dims}")
+    D = math.prod(dims)
+    if not 1 <= D <= LAYER_NORM_MAX:
+        raise ValueError(f"rows of {D} elements: layer_norm takes 1 to {LAYER_NORM_MAX}")
+    w, b = norm.weight, norm.bias
+    _lib.same_device(x, d=d, weight=w, bias=b)
+    for name, t in (("the addend", d), ("the weight", w), ("the bias", b)):
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError(f"{name} is {t.dtype}, x is {x.dtype}")
+    s = x
+    x, d, w, b = (None if t is None else _lib.dense(t) for t in (x, d, w, b))
+    h, r = _norm(x, d, w, b, D, float(norm.eps), True)
+    return h, s if d is None else r
+
+
+def _embed_forward(w, ids, scale):
+    out = w.new_empty(ids.shape + (w.shape[1],))
+    with _lib.device_of(w):
+        _lib.check(_lib.lib().lema_embedding(
+            w.data_ptr(), _lib.DTYPE_CODE[w.dtype], w.shape[0], w.shape[1], ids.data_ptr(), ids.numel(),
+            scale, out.data_ptr(), _lib.stream_of(w)))
     return out
+
+
+class _Embed(torch.autograd.Function):
+    """The lookup, and the table's gradient by sorted tokens (its sums have a fixed order)."""
+
+    @staticmethod
+    def forward(ctx, w, ids, scale, padding):
+        ctx.save_for_backward(ids)
+        ctx.table = *w.shape, scale, padding
+        return _embed_forward(w, ids, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        V, D, scale, padding = ctx.table
+        gy = _lib.dense(gy)
+        ids = _saved(ctx.saved_tensors[0], gy, torch.long)
+        gw = gy.new_empty(V, D)
+        L = _lib.lib()
+        n = L.lema_embedding_grad_workspace_bytes(ids.numel(), V, D)
+        ws = gy.new_empty(n, dtype=torch.uint8)
+        with _lib.device_of(gy):
+            _lib.check(L.lema_embedding_grad(
+                gy.data_ptr(), _lib.DTYPE_CODE[gy.dtype], ids.data_ptr(), ids.numel(), V, D, scale, padding,
+                gw.data_ptr(), ws.data_ptr(), n, _lib.stream_of(gy)))
+        return gw, None, None, None
+
+
+def embed(emb: nn.Embedding, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """emb(ids) * scale, rounded once, in float32, float16 or bfloat16. The ids must lie in
+    [0, vocab): an id outside it gives a zero row and no gradient, where nn.Embedding raises.
+
+    Differentiable in the table (`padding_idx` gets a zero gradient): the gradient adds up each
+    token's rows in a fixed order, in fp32. A table that nn.Embedding renormalises (max_norm), a
+    sparse gradient or one scaled by frequency, a table of more than 2^20 rows that wants a
+    gradient, and CPU tensors take the torch operations."""
+    w = emb.weight
+    grad = _needs_grad(w)
+    if not (w.is_cuda and ids.device == w.device and w.dtype in _lib.DTYPE_CODE and w.is_contiguous()
+            and ids.dtype in (torch.long, torch.int32) and emb.max_norm is None and w.numel()
+            and w.shape[1] <= 1 << 20
+            and not (grad and (emb.sparse or emb.scale_grad_by_freq or w.shape[0] > 1 << 20))):
+        y = emb(ids)
+        return y if scale == 1.0 else y * scale
+    ids = ids.to(torch.long).contiguous()
+    if grad:
+        return _Embed.apply(w, ids, float(scale), -1 if emb.padding_idx is None else emb.padding_idx)
+    return _embed_forward(w, ids, float(scale))
 
 
 def argmax_into(logits: torch.Tensor, out: torch.Tensor) -> None:
@@ -101,23 +252,79 @@ def argmax_into(logits: torch.Tensor, out: torch.Tensor) -> None:
                                            out.data_ptr(), 1, _lib.stream_of(logits)))
 
 
-def swiglu(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
-    if not (_fused(g, u) and g.numel() % 8 == 0):
-        return F.silu(g) * u
+def _swiglu_forward(g, u):
     out = torch.empty_like(g)
     _lib.check(_lib.lib().lema_swiglu_bf16(g.data_ptr(), u.data_ptr(), out.data_ptr(),
                                            g.numel(), _lib.stream_of(g)))
     return out
 
 
+class _SwiGLUProduct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g, u):
+        ctx.save_for_backward(g, u)
+        return _swiglu_forward(g, u)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        gy = _lib.dense(gy)
+        g, u = (_saved(t, gy, gy.dtype) for t in ctx.saved_tensors)
+        gg, gu = torch.empty_like(g), torch.empty_like(u)
+        with _lib.device_of(gy):
+            _lib.check(_lib.lib().lema_swiglu_grad_bf16(
+                g.data_ptr(), u.data_ptr(), gy.data_ptr(), gg.data_ptr(), gu.data_ptr(), g.numel(),
+                _lib.stream_of(gy)))
+        return gg, gu
+
+
+def swiglu(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
+    if not (_fused(g, u) and g.numel() % 8 == 0):
+        return F.silu(g) * u
+    return _SwiGLUProduct.apply(g, u) if _needs_grad(g, u) else _swiglu_forward(g, u)
+
+
+class _CrossEntropySum(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, y):
+        V = logits.shape[-1]
+        rows = logits.numel() // V
+        loss = logits.new_empty(rows, dtype=torch.float32)
+        stats = logits.new_empty(rows, 2, dtype=torch.float32)
+        with _lib.device_of(logits):
+            _lib.check(_lib.lib().lema_cross_entropy_stats_bf16(
+                logits.data_ptr(), rows, V, V, y.data_ptr(), loss.data_ptr(), stats.data_ptr(),
+                _lib.stream_of(logits)))
+        ctx.save_for_backward(logits, y, stats)
+        return loss.sum()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, y, stats = ctx.saved_tensors
+        logits, y, stats = (_saved(t, g, dt) for t, dt in
+                            ((logits, torch.bfloat16), (y, torch.long), (stats, torch.float32)))
+        V = logits.shape[-1]
+        rows = logits.numel() // V
+        grad, coef = torch.empty_like(logits), -g.reshape(1)
+        with _lib.device_of(g):
+            _lib.check(_lib.lib().lema_token_logprobs_grad(
+                logits.data_ptr(), _lib.BF16, rows, max(1, rows), V, 0, V, y.data_ptr(), None, 1.0,
+                stats.data_ptr(), coef.data_ptr(), max(1, rows), None, None, grad.data_ptr(),
+                _lib.stream_of(g)))
+        return grad, None
+
+
 def cross_entropy_sum(logits: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
-    """Sum over rows of logsumexp(logits) - logits[y] (fp32)."""
+    """Sum over rows of logsumexp(logits) - logits[y] (fp32), differentiable in the logits."""
     V = logits.shape[-1]
     if not (_fused(logits) and V % 8 == 0 and y.is_cuda):
         return F.cross_entropy(logits.float(), y, reduction="sum")
     rows = logits.numel() // V
-    loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
     yy = y.reshape(-1).to(torch.int64).contiguous()
+    if _needs_grad(logits):
+        return _CrossEntropySum.apply(logits, yy)
+    loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
     _lib.check(_lib.lib().lema_cross_entropy_bf16(
         logits.data_ptr(), rows, V, V, yy.data_ptr(), loss.data_ptr(), _lib.stream_of(logits)))
     return loss.sum()
@@ -132,16 +339,40 @@ def _skinny(x: torch.Tensor, weight: torch.Tensor) -> bool:
             and x.data_ptr() % 16 == 0 and weight.data_ptr() % 16 == 0)
 
 
+def _skinny_forward(x, w):
+    K, N = x.shape[-1], w.shape[0]
+    M = x.numel() // K
+    y = x.new_empty(x.shape[:-1] + (N,))
+    _lib.check(_lib.lib().lema_skinny_gemm_bf16(
+        x.data_ptr(), K, w.data_ptr(), K, y.data_ptr(), N, M, N, K, _lib.stream_of(x)))
+    return y
+
+
+class _SkinnyLinear(torch.autograd.Function):
+    """The skinny product where a gradient is wanted: the same y, nn.Linear's gradients."""
+
+    @staticmethod
+    def forward(ctx, x, w):
+        ctx.save_for_backward(x, w)
+        return _skinny_forward(x, w)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, w = ctx.saved_tensors
+        g2 = gy.reshape(-1, gy.shape[-1])
+        gx = (g2 @ w).view(x.shape) if ctx.needs_input_grad[0] else None
+        gw = g2.t() @ x.reshape(-1, x.shape[-1]) if ctx.needs_input_grad[1] else None
+        return gx, gw
+
+
 def linear(x: torch.Tensor, lin: nn.Linear) -> torch.Tensor:
     """lin(x); a decode-shaped product (<= 32 rows, bf16) on the skinny MFMA kernel."""
     if not _skinny(x, lin.weight):
         return lin(x)
-    K, N = x.shape[-1], lin.weight.shape[0]
-    M = x.numel() // K
-    y = x.new_empty(x.shape[:-1] + (N,))
-    _lib.check(_lib.lib().lema_skinny_gemm_bf16(
-        x.data_ptr(), K, lin.weight.data_ptr(), K, y.data_ptr(), N, M, N, K, _lib.stream_of(x)))
-    return y
+    if _needs_grad(x, lin.weight):
+        return _SkinnyLinear.apply(x, lin.weight)
+    return _skinny_forward(x, lin.weight)
 
 
 def project_codes(x: torch.Tensor, lin: nn.Linear, d: int, code_dtype: torch.dtype):
@@ -310,7 +541,8 @@ class SwiGLU(nn.Module):
         the residual in its epilogue; on longer bf16 inputs without autograd the down GEMM
         accumulates into `residual` itself, which is then returned."""
         g, u, dn = self.gate.weight, self.up.weight, self.down.weight
-        if _skinny(x, g) and g.shape == u.shape and u.data_ptr() % 16 == 0 and u.is_contiguous():
+        if _skinny(x, g) and g.shape == u.shape and u.data_ptr() % 16 == 0 and u.is_contiguous() \
+                and not _needs_grad(x, g, u, dn, residual):
             K, N = x.shape[-1], g.shape[0]
             M = x.numel() // K
             a = x.new_empty(x.shape[:-1] + (N,))
@@ -465,8 +697,10 @@ class Block(nn.Module):
     def forward(self, x, store=None):
         if store is not None:
             pre, post = self.seg or (self.gpu_pre, self.gpu_post)
-            qc, kc, v = pre(x)
-            return post(x, store.exchange(qc, kc, v))
+            # the exchange has no gradient, and neither do the fused bf16 launches around it
+            with torch.no_grad() if x.is_cuda and x.dtype is torch.bfloat16 else contextlib.nullcontext():
+                qc, kc, v = pre(x)
+                return post(x, store.exchange(qc, kc, v))
         h, x = rms_norm(x, self.norm2, self.attn(self.pre_attn(x)))
         return self.mlp(h, residual=x)
 
@@ -528,16 +762,20 @@ class Transformer(nn.Module):
         if cache is not None and not (self.lema_layers()
                                       and all(a.hard for a in self.lema_layers())):
             raise ValueError("a cache needs an all-LEMA model in hard mode")
-        x = self.tok_emb(idx)
+        x = self._embed(idx) if cache is None else self.tok_emb(idx)
         for li, blk in enumerate(self.blocks):
             x = blk(x, store=(cache.layer(li) if cache is not None else None))
         if cache is not None:
             cache.t += idx.shape[-1]
         return linear(rms_norm(x, self.norm_f)[0], self.lm_head) if return_logits else None
 
+    def _embed(self, idx):
+        """The token rows: `embed`, whose gradient sorts the tokens, where one is wanted."""
+        return embed(self.tok_emb, idx) if _needs_grad(self.tok_emb.weight) else self.tok_emb(idx)
+
     def hidden(self, idx):
         """The final normalised hidden states (the input of lm_head), without a cache."""
-        x = self.tok_emb(idx)
+        x = self._embed(idx)
         for blk in self.blocks:
             x = blk(x)
         return rms_norm(x, self.norm_f)[0]
@@ -552,7 +790,7 @@ class Transformer(nn.Module):
 def lm_loss(model: Transformer, x: torch.Tensor, y: torch.Tensor, chunk: int = 4096):
     """Mean next-token cross-entropy without holding the full `[B, T, vocab]` logits: the
     head and the loss run `chunk` positions at a time on the final hidden states, in fp32
-    (code/lema/train.py:131-152, forward only). At B4 T16384 with a 50,304-word vocabulary,
+    (code/lema/train.py:131-152). Differentiable; a backward keeps the chunks' logits until then. At B4 T16384 with a 50,304-word vocabulary,
     chunks of 4096 positions (head GEMMs of 16,384 rows, 1.65 GB of bf16 logits at a time)
     took the whole forward from 119.9-120.4 to 118.2-118.8 ms against chunks of 1024."""
     h = model.hidden(x)
