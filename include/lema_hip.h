@@ -39,6 +39,11 @@ const char* lema_last_error(void);
 /* The version of this C ABI (1). No counterpart in the reference. */
 int lema_abi_version(void);
 
+/* Which graph capture `stream` records into: an id above 0, 0 for none, -1 where that cannot be
+ * told. Work recorded in one capture is replayed together and in order. No counterpart in the
+ * reference. */
+int64_t lema_capture_id(void* stream);
+
 /* dst[0, bytes) = src[0, bytes) on the device (bytes a multiple of 16, both pointers 16-byte
  * aligned). No counterpart in the reference: the benchmark's roofline compares the kernels'
  * HBM rates with this copy's, the streaming rate the memory reaches in practice. */
@@ -293,11 +298,13 @@ int lema_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t
 /* The logits' gradient where each row's lp has the gradient c = coef[r / per] * *scale0 * *scale1
  * (device scalars, NULL = 1): grad[r, j] = c / temperature * ([j = target[r]] - softmax[j]), in
  * fp32, rounded once; grad contiguous [rows, V]. Rows with c = 0 and rows that the mask leaves
- * out are not read: their gradient is zero. */
+ * out are not read: their gradient is zero. unit_done != 0: grad already holds the gradient for
+ * *scale0 = 1 (lema_policy_loss wrote it) and is left as it is where *scale0 is 1. */
 int lema_token_logprobs_grad(const void* logits, int32_t dtype, int64_t rows, int64_t inner, int64_t V,
                              int64_t so, int64_t si, const int64_t* target, const uint8_t* mask,
                              float temperature, const float* stats, const float* coef, int64_t per,
-                             const float* scale0, const float* scale1, void* grad, void* stream);
+                             const float* scale0, const float* scale1, int32_t unit_done, void* grad,
+                             void* stream);
 
 /* Clipped policy loss of sampled tokens, and what its gradient needs. Per row, with lp and stats as
  * above, ratio = e^(lp - old_lp) and A = advantage:
@@ -305,12 +312,16 @@ int lema_token_logprobs_grad(const void* logits, int32_t dtype, int64_t rows, in
  *          + kl (e^(ref_lp - lp) - (ref_lp - lp) - 1)        (ref_lp NULL or kl 0: without)
  *   coef = d term / d lp;  both 0 for rows that the mask leaves out
  * loss = mean of the counted rows' terms (0 without any), inv_n = 1 / counted rows: the gradient
- * of the loss is lema_token_logprobs_grad with coef, per = 1 and inv_n as a scale. */
+ * of the loss is lema_token_logprobs_grad with coef, per = 1 and inv_n as a scale.
+ *   grad  NULL, or contiguous [rows, V] of `dtype` that receives that gradient for a gradient of
+ *         1 of the loss: rows of up to 256 KB that start on the same bytes of a 16-byte piece as
+ *         grad's are then read once for both */
 int lema_policy_loss(const void* logits, int32_t dtype, int64_t rows, int64_t inner, int64_t V,
                      int64_t so, int64_t si, const int64_t* target, const uint8_t* mask,
                      float temperature, const float* old_lp, const float* advantage,
                      const float* ref_lp, float clip_low, float clip_high, float kl, float* lp,
-                     float* stats, float* term, float* coef, float* loss, float* inv_n, void* stream);
+                     float* stats, float* term, float* coef, float* loss, float* inv_n, void* grad,
+                     void* stream);
 
 /* Paired preference loss from token log-probabilities lp64 [2 * pairs, T], the chosen answers
  * first, and the reference's ref_lp: with s the sum of an answer's counted lp64 - ref_lp,

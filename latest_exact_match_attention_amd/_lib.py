@@ -10,6 +10,7 @@ import weakref
 from pathlib import Path
 
 import torch
+from torch.autograd.function import once_differentiable
 
 LIB_PATH = Path(__file__).resolve().parent / "liblema_hip.so"
 # the diagnostics build (decode-step clock readings); loaded only when a caller asks for it
@@ -33,6 +34,7 @@ _f32 = ctypes.c_float
 PROTOTYPES = {
     "lema_last_error": ([], ctypes.c_char_p),
     "lema_abi_version": ([], ctypes.c_int),
+    "lema_capture_id": ([_p], ctypes.c_int64),
     "lema_device_copy": ([_p, _p, _i64, _p], ctypes.c_int),
     "lema_pack_codes": ([_p, _i32, _i64, _i64, _i64, _i32, _i64, _i64, _i64, _p, _i32, _p],
                         ctypes.c_int),
@@ -73,9 +75,9 @@ PROTOTYPES = {
     "lema_token_logprobs": ([_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _f32, _p, _p, _p, _p],
                             ctypes.c_int),
     "lema_token_logprobs_grad": ([_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _f32, _p, _p, _i64,
-                                  _p, _p, _p, _p], ctypes.c_int),
+                                  _p, _p, _i32, _p, _p], ctypes.c_int),
     "lema_policy_loss": ([_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _f32, _p, _p, _p, _f32, _f32,
-                          _f32, _p, _p, _p, _p, _p, _p, _p], ctypes.c_int),
+                          _f32, _p, _p, _p, _p, _p, _p, _p, _p], ctypes.c_int),
     "lema_preference_loss": ([_p, _p, _p, _i64, _i64, _f32, _f32, _p, _p, _p, _p], ctypes.c_int),
     "lema_skinny_gemm_bf16": ([_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _p], ctypes.c_int),
     "lema_skinny_pack_bf16": ([_p, _i64, _p, _i64, _i64, _i64, _i64, _i32, _i64, _p, _i32, _p],
@@ -185,7 +187,25 @@ def same_device(t: torch.Tensor, **others) -> None:
 
 def dense(t: torch.Tensor) -> torch.Tensor:
     """t as the kernels read it: contiguous, its values the ones in memory."""
-    return t.resolve_neg().contiguous()
+    return t.contiguous() if not t.is_neg() else t.resolve_neg().contiguous()
+
+
+def saved(t: torch.Tensor, like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A saved tensor as it was saved, on `like`'s device: a saved-tensor hook may bring it back in
+    another form."""
+    if t.dtype is dtype and t.device == like.device and t.is_contiguous() and not t.is_neg():
+        return t
+    return dense(t.to(device=like.device, dtype=dtype))
+
+
+def once(backward):
+    """A Function's backward whose gradients have none themselves, as torch's once_differentiable
+    does it, but at no cost (that takes 6 us) where nobody records them."""
+    recorded = once_differentiable(backward)
+
+    def fn(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return fn
 
 
 # ---- host memory the GPU works on in place (a store table in host RAM) ----

@@ -22,6 +22,16 @@ extern "C" const char* lema_last_error(void) { return lema::g_error; }
 
 extern "C" int lema_abi_version(void) { return 1; }
 
+extern "C" int64_t lema_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return -1;
+  }
+  return status == hipStreamCaptureStatusNone ? 0 : static_cast<int64_t>(id);
+}
+
 namespace lema {
 namespace {
 

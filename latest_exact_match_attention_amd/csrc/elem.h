@@ -14,7 +14,7 @@ __device__ __forceinline__ float to_f32(Bf16 v) {
   return __uint_as_float(static_cast<uint32_t>(v.bits) << 16);
 }
 
-// Round to nearest even; a NaN becomes the canonical quiet one in bf16.
+// Round to nearest even (in bf16 gfx950's own conversion, a pair in one instruction).
 template <typename T>
 __device__ __forceinline__ T from_f32(float f);
 template <>
@@ -27,9 +27,7 @@ __device__ __forceinline__ _Float16 from_f32<_Float16>(float f) {
 }
 template <>
 __device__ __forceinline__ Bf16 from_f32<Bf16>(float f) {
-  const uint32_t b = __float_as_uint(f);
-  if ((b & 0x7F800000u) == 0x7F800000u && (b & 0x007FFFFFu) != 0) return Bf16{0x7FC0u};
-  return Bf16{static_cast<uint16_t>((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16)};
+  return Bf16{__builtin_bit_cast(uint16_t, static_cast<__bf16>(f))};
 }
 
 template <typename T>

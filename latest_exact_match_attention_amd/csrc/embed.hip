@@ -9,7 +9,7 @@
 //            (the token's high bits);
 //   scatter  each span puts its positions, in order, into the buckets;
 //   order    each bucket orders its positions by token, and notes where each token's start;
-//   sum      a wavefront per (token, 512 columns) adds up to 64 rows. A longer list would
+//   sum      a wavefront per (token, 512 columns) adds up to 32 rows. A longer list would
 //            keep one wavefront busy while the others end, so its whole tiles of 32 positions are
 //            summed by wavefronts of their own, in the same launch, in fp32;
 //   join     a workgroup per (long list, 512 columns) adds its tiles and its ragged ends.
@@ -24,7 +24,7 @@ namespace {
 constexpr int kBuckets = 1024;      // at most, of 1 << row_bits tokens each
 constexpr int kMaxRowBits = 10;     // so at most 2^20 tokens
 constexpr int kSpanStep = 1024;     // a span is a multiple of it: 16 wavefronts of 64
-constexpr int kTile = 32, kLong = 64;
+constexpr int kTile = 32, kLong = 32;
 constexpr int kCols = 512;          // columns of a wavefront, 8 a lane
 
 __device__ __forceinline__ int wave_index() {
@@ -161,7 +161,6 @@ __device__ __forceinline__ uint32_t take_place(uint32_t* cursors, uint32_t digit
 __global__ __launch_bounds__(1024) void embed_count_kernel(Order o) {
   __shared__ uint32_t hist[kBuckets];
   hist[threadIdx.x] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *o.long_count = 0;
   __syncthreads();
   const int64_t at = blockIdx.x * o.span, end = min(at + o.span, o.n);
   for (int64_t i = at + threadIdx.x; i < end; i += 1024) {
@@ -205,14 +204,25 @@ __global__ __launch_bounds__(1024) void embed_scatter_kernel(Order o) {
   }
   // thread t: bucket t's positions in all spans, and in the spans before this one
   uint32_t all = 0, before = 0;
-#pragma unroll 8
-  for (int s = 0; s < o.spans; ++s) {
-    const uint32_t c = o.counts[static_cast<int64_t>(s) * kBuckets + t];
-    all += c;
-    before += s < static_cast<int>(blockIdx.x) ? c : 0u;
+  if (o.spans == 1) {  // not counted before: the sixteenths just counted are all there is
+    __syncthreads();
+    for (int k = 0; k < 16; ++k) all += cur[k][t];
+  } else {
+    for (int s0 = 0; s0 < o.spans; s0 += 32) {
+      uint32_t c[32];
+#pragma unroll
+      for (int u = 0; u < 32; ++u)
+        c[u] = o.counts[static_cast<int64_t>(s0 + u < o.spans ? s0 + u : s0) * kBuckets + t];
+#pragma unroll
+      for (int u = 0; u < 32; ++u) {
+        if (s0 + u < o.spans) all += c[u];
+        if (s0 + u < static_cast<int>(blockIdx.x)) before += c[u];
+      }
+    }
   }
   uint32_t base = group_scan<16>(all, red);  // its barrier also ends the counting above
   if (blockIdx.x == 0) {
+    if (t == 0) *o.long_count = 0;
     o.bucket_at[t] = base;
     if (t == kBuckets - 1) o.bucket_at[kBuckets] = base + all;
   }
@@ -236,126 +246,206 @@ __global__ __launch_bounds__(1024) void embed_scatter_kernel(Order o) {
 
 // One workgroup per bucket: its positions ordered by token, and where each token's start.
 __global__ __launch_bounds__(512) void embed_order_kernel(Order o) {
-  __shared__ uint32_t cur[8][1 << kMaxRowBits];
+  extern __shared__ uint32_t cursors[];  // [8][rows]
   __shared__ uint32_t red[8];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   const int rows = 1 << o.row_bits;
+  uint32_t* const cur = cursors + w * rows;
   const uint32_t b0 = o.bucket_at[blockIdx.x], b1 = o.bucket_at[blockIdx.x + 1];
   const uint32_t part = ((b1 - b0) / 512 + 1) * 64;  // 8 parts cover the bucket
   const uint32_t at = min(b0 + w * part, b1), end = min(at + part, b1);
-  for (int k = t; k < 8 * rows; k += 512) cur[k / rows][k % rows] = 0;
+  for (int k = t; k < 8 * rows; k += 512) cursors[k] = 0;
   __syncthreads();
-  for (uint32_t i = at + lane; i < end; i += 64) atomicAdd(&cur[w][o.item_id[i] & (rows - 1)], 1u);
+  // 8 batches of 64 in flight: a bucket with a frequent token is long
+  for (uint32_t i0 = at; i0 < end; i0 += 8 * 64) {
+    uint32_t id[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) id[u] = o.item_id[min(i0 + u * 64 + lane, end - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + u * 64 + lane < end) atomicAdd(&cur[id[u] & (rows - 1)], 1u);
+  }
   __syncthreads();
   uint32_t mine[2] = {0, 0};  // tokens 2 t and 2 t + 1 of the bucket
   for (int j = 0; j < 2; ++j)
     if (2 * t + j < rows)
-      for (int k = 0; k < 8; ++k) mine[j] += cur[k][2 * t + j];
+      for (int k = 0; k < 8; ++k) mine[j] += cursors[k * rows + 2 * t + j];
   uint32_t base = b0 + group_scan<8>(mine[0] + mine[1], red);
   for (int j = 0; j < 2; ++j) {
     const int r = 2 * t + j;
+    if (r >= rows) break;
     const int64_t v = (static_cast<int64_t>(blockIdx.x) << o.row_bits) + r;
-    if (r < rows) {
-      if (v < o.vocab) {
-        o.start[v] = base;
-        if (v == o.vocab - 1) o.start[o.vocab] = b1;
-        if (mine[j] > kLong) o.long_list[atomicAdd(o.long_count, 1u)] = static_cast<uint32_t>(v);
-      }
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t c = cur[k][r];
-        cur[k][r] = base;
-        base += c;
-      }
+    if (v < o.vocab) {
+      o.start[v] = base;
+      if (v == o.vocab - 1) o.start[o.vocab] = b1;
+      if (mine[j] > kLong) o.long_list[atomicAdd(o.long_count, 1u)] = static_cast<uint32_t>(v);
+    }
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t c = cursors[k * rows + r];
+      cursors[k * rows + r] = base;
+      base += c;
     }
   }
   __syncthreads();
-  for (uint32_t i0 = at; i0 < end; i0 += 64) {
-    const bool live = i0 + lane < end;
-    const uint32_t id = live ? o.item_id[i0 + lane] : 0u;
-    const uint32_t place = take_place(cur[w], id & (rows - 1), live, o.row_bits, lane);
-    if (live) {
-      o.perm[place] = o.item_pos[i0 + lane];
-      o.token[place] = id;
+  for (uint32_t i0 = at; i0 < end; i0 += 8 * 64) {
+    uint32_t id[8], pos[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t i = min(i0 + u * 64 + lane, end - 1);
+      id[u] = o.item_id[i];
+      pos[u] = o.item_pos[i];
+    }
+    for (int u = 0; u < 8; ++u) {
+      if (i0 + u * 64 >= end) break;
+      const bool live = i0 + u * 64 + lane < end;
+      const uint32_t place = take_place(cur, id[u] & (rows - 1), live, o.row_bits, lane);
+      if (live) {
+        o.perm[place] = pos[u];
+        o.token[place] = id[u];
+      }
     }
   }
 }
 
-// acc += gy rows perm[j], j in [j0, j1), in order: 64 positions read at once, 4 rows in flight.
-template <typename T, bool kVec>
+// C slices of 512 columns of a row, as they come from memory.
+template <typename T, int C, bool kVec>
+struct RawSlices {
+  Piece<T> q[C * 8 / kPiece<T>];
+
+  __device__ __forceinline__ void fetch(const T* row, int64_t c0, int64_t D, int lane) {
+    constexpr int n = kPiece<T>;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if constexpr (kVec) {
+        const int64_t e = c0 + c * kCols + lane * 8;
+#pragma unroll
+        for (int i = 0; i < 8 / n; ++i)
+          q[c * 8 / n + i].raw =
+              e < D ? *reinterpret_cast<const u32x4*>(row + e + i * n) : u32x4{0, 0, 0, 0};
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int64_t e = c0 + c * kCols + k * 64 + lane;
+          q[(c * 8 + k) / n].e[k % n] = e < D ? row[e] : T{};
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float at(int k) const { return to_f32(q[k / kPiece<T>].e[k % kPiece<T>]); }
+};
+
+template <typename T, int C, bool kVec>
+__device__ __forceinline__ void store_slices(T* row, int64_t c0, int64_t D, int lane, const float (&v)[C * 8]) {
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    float part[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) part[k] = v[c * 8 + k];
+    store_slice<T, kVec>(row, c0 + c * kCols, D, lane, part);
+  }
+}
+
+// acc += gy rows perm[j], j in [j0, j1), in order: 64 positions read at once, 4 or 8 rows in flight.
+template <typename T, int C, bool kVec>
 __device__ __forceinline__ void add_rows(const T* gy, const uint32_t* perm, uint32_t j0, uint32_t j1,
-                                         int64_t c0, int64_t D, int lane, float (&acc)[8]) {
+                                         int64_t c0, int64_t D, int lane, float (&acc)[C * 8]) {
   for (uint32_t j = j0; j < j1; j += 64) {
     const int m = min(64u, j1 - j);
     const uint32_t pos = perm[j + min(lane, m - 1)];
-    for (int i = 0; i < m; i += 4) {
-      float v[4][8];
+    constexpr int kRows = C == 1 ? 8 : 4;
+    for (int i = 0; i < m; i += kRows) {
+      RawSlices<T, C, kVec> v[kRows];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kRows; ++u) {
         const uint32_t p = __builtin_amdgcn_readlane(pos, min(i + u, m - 1));
-        load_slice<T, kVec>(gy + static_cast<int64_t>(p) * D, c0, D, lane, v[u]);
+        if (u == 0 || i + u < m) v[u].fetch(gy + static_cast<int64_t>(p) * D, c0, D, lane);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < kRows; ++u)
+        if (u == 0 || i + u < m) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] += i + u < m ? v[u][k] : 0.0f;
+          for (int k = 0; k < C * 8; ++k) acc[k] += v[u].at(k);
+        }
     }
   }
 }
 
-// One wavefront per (tile or token, 512 columns): the tiles come first. partial: [tiles, D].
-template <typename T, bool kVec>
+// One wavefront per (tile or token, C slices of 512 columns): the tiles come first. partial: [tiles, D].
+template <typename T, int C, bool kVec>
 __global__ __launch_bounds__(256) void embed_sum_kernel(Order o, const T* gy, int64_t D, int slices,
                                                         int64_t tiles, float scale, float* partial,
                                                         T* gw) {
   const int lane = threadIdx.x & 63;
   const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + wave_index();
-  const int64_t item = u / slices, c0 = (u - item * slices) * kCols;
+  const int64_t item = u / slices, c0 = (u - item * slices) * C * kCols;
   if (item >= tiles + o.vocab) return;
-  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  float acc[C * 8];
+#pragma unroll
+  for (int k = 0; k < C * 8; ++k) acc[k] = 0.0f;
   if (item < tiles) {
     const uint32_t j0 = static_cast<uint32_t>(item) * kTile;
     if (j0 + kTile > o.start[o.vocab]) return;
     const uint32_t v = o.token[j0];
     if (o.token[j0 + kTile - 1] != v || o.start[v + 1] - o.start[v] <= kLong) return;
-    add_rows<T, kVec>(gy, o.perm, j0, j0 + kTile, c0, D, lane, acc);
-    store_slice<float, kVec>(partial + item * D, c0, D, lane, acc);
+    add_rows<T, C, kVec>(gy, o.perm, j0, j0 + kTile, c0, D, lane, acc);
+    store_slices<float, C, kVec>(partial + item * D, c0, D, lane, acc);
   } else {
     const int64_t v = item - tiles;
     const uint32_t j0 = o.start[v], j1 = o.start[v + 1];
     if (j1 - j0 > kLong) return;
-    add_rows<T, kVec>(gy, o.perm, j0, j1, c0, D, lane, acc);
+    add_rows<T, C, kVec>(gy, o.perm, j0, j1, c0, D, lane, acc);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) acc[k] *= scale;
-    store_slice<T, kVec>(gw + v * D, c0, D, lane, acc);
+    for (int k = 0; k < C * 8; ++k) acc[k] *= scale;
+    store_slices<T, C, kVec>(gw + v * D, c0, D, lane, acc);
   }
 }
 
-// One workgroup per (long list, 512 columns). A list of more than 64 holds a whole tile at least.
+// One workgroup per (long list, 512 columns): the positions before the first whole tile, the tiles'
+// sums and the positions after the last one, each dealt out to the 16 wavefronts, the tiles 8 at a time
+// in flight: the most frequent token of 65,536 has about 250.
 template <typename T, bool kVec>
-__global__ __launch_bounds__(256) void embed_join_kernel(Order o, const T* gy, int64_t D, float scale,
-                                                         const float* partial, T* gw) {
-  __shared__ float sums[4][8][64];
+__global__ __launch_bounds__(1024) void embed_join_kernel(Order o, const T* gy, int64_t D, float scale,
+                                                          const float* partial, T* gw) {
+  __shared__ float sums[16][8][64];
   if (blockIdx.x >= *o.long_count) return;
-  const int lane = threadIdx.x & 63, w = wave_index();
+  const int lane = threadIdx.x & 63;
+  const uint32_t w = wave_index();
   const int64_t v = o.long_list[blockIdx.x], c0 = static_cast<int64_t>(blockIdx.y) * kCols;
   const uint32_t j0 = o.start[v], j1 = o.start[v + 1];
-  const uint32_t t0 = (j0 + kTile - 1) / kTile, t1 = j1 / kTile;
+  const uint32_t t0 = (j0 + kTile - 1) / kTile, t1 = max(j1 / kTile, t0);
+  const uint32_t head = min(t0 * kTile, j1), tail = max(t1 * kTile, head);
   float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (w == 0) add_rows<T, kVec>(gy, o.perm, j0, t0 * kTile, c0, D, lane, acc);
-  if (w == 1) add_rows<T, kVec>(gy, o.perm, t1 * kTile, j1, c0, D, lane, acc);
-  for (uint32_t t = t0 + w; t < t1; t += 4) {
-    float p[8];
-    load_slice<float, kVec>(partial + static_cast<int64_t>(t) * D, c0, D, lane, p);
+  constexpr uint32_t kShare = kTile / 16;  // of an end's positions
+  add_rows<T, 1, kVec>(gy, o.perm, min(j0 + w * kShare, head), min(j0 + (w + 1) * kShare, head), c0, D,
+                       lane, acc);
+  for (uint32_t t = t0 + w; t < t1; t += 16 * 8) {
+    RawSlices<float, 1, kVec> p[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) acc[k] += p[k];
+    for (int u = 0; u < 8; ++u)
+      p[u].fetch(partial + static_cast<int64_t>(t + 16 * u < t1 ? t + 16 * u : t) * D, c0, D, lane);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (t + 16 * u < t1) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += p[u].at(k);
+      }
   }
+  add_rows<T, 1, kVec>(gy, o.perm, min(tail + w * kShare, j1), min(tail + (w + 1) * kShare, j1), c0, D,
+                       lane, acc);
 #pragma unroll
   for (int k = 0; k < 8; ++k) sums[w][k][lane] = acc[k];
   __syncthreads();
+  // 8 wavefronts add up a column of each lane's eight each, then the first one writes them
+  if (w < 8) {
+    float s = sums[0][w][lane];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += sums[i][w][lane];
+    sums[0][w][lane] = s * scale;
+  }
+  __syncthreads();
   if (w != 0) return;
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    acc[k] = (acc[k] + sums[1][k][lane] + sums[2][k][lane] + sums[3][k][lane]) * scale;
+  for (int k = 0; k < 8; ++k) acc[k] = sums[0][k][lane];
   store_slice<T, kVec>(gw + v * D, c0, D, lane, acc);
 }
 
@@ -464,22 +554,26 @@ extern "C" int lema_embedding_grad(const void* gy, int32_t dtype, const int64_t*
   o.ids = ids;
   o.padding = padding;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t slices = (D + kCols - 1) / kCols, tiles = n / kTile, longest = n / (kLong + 1);
+  const int64_t cols = (D + kCols - 1) / kCols, tiles = n / kTile, longest = n / (kLong + 1);
+  // a wavefront takes up to 3 slices: its chain of reads (start, positions, rows) is then shared
+  const int64_t per = cols < 3 ? cols : 3, slices = (cols + per - 1) / per;
   const int64_t grid = ((tiles + vocab) * slices + 3) / 4;
   LEMA_REQUIRE(grid < (int64_t(1) << 31), "table [%lld, %lld] is too large", (long long)vocab,
                (long long)D);
-  embed_count_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
+  if (o.spans > 1) embed_count_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
   embed_scatter_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
-  embed_order_kernel<<<dim3(o.buckets), dim3(512), 0, st>>>(o);
+  embed_order_kernel<<<dim3(o.buckets), dim3(512), 8 * 4 << o.row_bits, st>>>(o);
   const bool vec = D % 8 == 0 && aligned(gy, 16) && aligned(gw, 16);
   for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const auto sum = vec ? embed_sum_kernel<T, true> : embed_sum_kernel<T, false>;
+    const auto sum = per == 1   ? (vec ? embed_sum_kernel<T, 1, true> : embed_sum_kernel<T, 1, false>)
+                     : per == 2 ? (vec ? embed_sum_kernel<T, 2, true> : embed_sum_kernel<T, 2, false>)
+                                : (vec ? embed_sum_kernel<T, 3, true> : embed_sum_kernel<T, 3, false>);
     sum<<<dim3(grid), dim3(256), 0, st>>>(o, static_cast<const T*>(gy), D, static_cast<int>(slices),
                                           tiles, scale, partial, static_cast<T*>(gw));
     if (longest > 0) {
       const auto join = vec ? embed_join_kernel<T, true> : embed_join_kernel<T, false>;
-      join<<<dim3(longest, slices), dim3(256), 0, st>>>(o, static_cast<const T*>(gy), D, scale, partial,
+      join<<<dim3(longest, cols), dim3(1024), 0, st>>>(o, static_cast<const T*>(gy), D, scale, partial,
                                                         static_cast<T*>(gw));
     }
   });

@@ -30,27 +30,40 @@ __device__ __forceinline__ int elem_at(int s, int k, int lane) {
   return kVec ? (s * W * 64 + lane) * 8 + k : (s * 8 + k) * W * 64 + lane;
 }
 
+// A row's elements as they come from memory, so that a row can be on its way while the one before
+// it is worked on.
 template <typename T, int W, int S, bool kVec>
-__device__ __forceinline__ void load_row(const T* p, int D, int lane, float (&v)[S * 8]) {
+struct RawRow {
+  Piece<T> q[S * 8 / kPiece<T>];
+
+  __device__ __forceinline__ void fetch(const T* p, int D, int lane) {
+    constexpr int n = kPiece<T>;
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    if constexpr (kVec) {
-      const int e = elem_at<W, true>(s, 0, lane);
-      constexpr int n = kPiece<T>;
-      Piece<T> q[8 / n];
+    for (int s = 0; s < S; ++s) {
+      if constexpr (kVec) {
+        const int e = elem_at<W, true>(s, 0, lane);
 #pragma unroll
-      for (int i = 0; i < 8 / n; ++i)
-        q[i].raw = e < D ? *reinterpret_cast<const u32x4*>(p + e + i * n) : u32x4{0, 0, 0, 0};
+        for (int i = 0; i < 8 / n; ++i)
+          q[s * 8 / n + i].raw =
+              e < D ? *reinterpret_cast<const u32x4*>(p + e + i * n) : u32x4{0, 0, 0, 0};
+      } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[s * 8 + k] = to_f32(q[k / n].e[k % n]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int e = elem_at<W, false>(s, k, lane);
-        v[s * 8 + k] = e < D ? to_f32(p[e]) : 0.0f;
+        for (int k = 0; k < 8; ++k) {
+          const int e = elem_at<W, false>(s, k, lane);
+          q[(s * 8 + k) / n].e[k % n] = e < D ? p[e] : T{};
+        }
       }
     }
   }
+  __device__ __forceinline__ float at(int k) const { return to_f32(q[k / kPiece<T>].e[k % kPiece<T>]); }
+};
+
+template <typename T, int W, int S, bool kVec>
+__device__ __forceinline__ void load_row(const T* p, int D, int lane, float (&v)[S * 8]) {
+  RawRow<T, W, S, kVec> r;
+  r.fetch(p, D, lane);
+#pragma unroll
+  for (int k = 0; k < S * 8; ++k) v[k] = r.at(k);
 }
 
 template <typename T, int W, int S, bool kVec>
@@ -165,11 +178,27 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
 #pragma unroll
   for (int k = 0; k < S * 8; ++k) gw[k] = gb[k] = 0.0f, wv[k] = 1.0f;
   if (w != nullptr) load_row<T, W, S, kVec>(w, D, lane, wv);
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kSlots + slot; row < rows;
-       row += static_cast<int64_t>(gridDim.x) * kSlots) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kSlots;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kSlots + slot;
+  RawRow<T, W, S, kVec> next_v, next_g, next_gs;
+  const bool add = gx != nullptr && gs != nullptr;
+  const auto fetch = [&](int64_t r) {
+    next_v.fetch(s_in + r * D, D, lane);
+    next_g.fetch(gh + r * D, D, lane);
+    if (add) next_gs.fetch(gs + r * D, D, lane);
+  };
+  constexpr bool kAhead = S == 1;  // with more, the registers of the row on its way spill
+  if (kAhead && row < rows) fetch(row);
+  for (; row < rows; row += step) {
+    if (!kAhead) fetch(row);
     float v[S * 8], g[S * 8];
-    load_row<T, W, S, kVec>(s_in + row * D, D, lane, v);
-    load_row<T, W, S, kVec>(gh + row * D, D, lane, g);
+    const RawRow<T, W, S, kVec> gs_row = next_gs;
+#pragma unroll
+    for (int k = 0; k < S * 8; ++k) {
+      v[k] = next_v.at(k);
+      g[k] = next_g.at(k);
+    }
+    if (kAhead && row + step < rows) fetch(row + step);
     if constexpr (kCenter) {
       float sum[1] = {0.0f};
 #pragma unroll
@@ -201,10 +230,9 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
       v[k] = r * (g[k] * wv[k] - c1 - z * c2);
     }
     if (gx != nullptr) {
-      if (gs != nullptr) {
-        load_row<T, W, S, kVec>(gs + row * D, D, lane, g);
+      if (add) {
 #pragma unroll
-        for (int k = 0; k < S * 8; ++k) v[k] += g[k];
+        for (int k = 0; k < S * 8; ++k) v[k] += gs_row.at(k);
       }
       store_row<T, W, S, kVec>(gx + row * D, D, lane, v);
     }
@@ -240,26 +268,37 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
   }
 }
 
-// out[e] = sum over `parts` of partial[p, e]; blockIdx.y picks the weight's or the bias's. 16
-// groups of 16 columns' threads each take every 16th part.
+// out[e] = sum over `parts` of partial[p, e]; blockIdx.y picks the weight's or the bias's. 64
+// groups of 16 columns' threads each take every 64th part, 8 parts in flight: the partial sums
+// are a few MB in L2 and the Infinity Cache, and a thread that waits for each of them in turn took
+// 25 us for 1024 parts of 1536.
 template <typename T>
-__global__ __launch_bounds__(256) void norm_weight_kernel(const float* partial, int parts, int D,
-                                                          T* gw, T* gb) {
-  __shared__ float sums[16][17];
+__global__ __launch_bounds__(1024) void norm_weight_kernel(const float* partial, int parts, int D,
+                                                           T* gw, T* gb) {
+  __shared__ float sums[64][17];
   T* out = blockIdx.y ? gb : gw;
   if (out == nullptr) return;
   const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
   const int e = blockIdx.x * 16 + c;
-  const float* p = partial + static_cast<int64_t>(blockIdx.y) * parts * D + e;
+  const float* p = partial + static_cast<int64_t>(blockIdx.y) * parts * D + (e < D ? e : 0);
   float t = 0.0f;
-  if (e < D)
-    for (int i = q; i < parts; i += 16) t += p[static_cast<int64_t>(i) * D];
+  for (int i = q; i < parts; i += 64 * 8) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int at = i + u * 64;
+      v[u] = p[static_cast<int64_t>(at < parts ? at : q) * D];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t += i + u * 64 < parts ? v[u] : 0.0f;
+  }
   sums[q][c] = t;
   __syncthreads();
-  if (q == 0 && e < D) {
-    for (int i = 1; i < 16; ++i) t += sums[i][c];
-    out[e] = from_f32<T>(t);
+  for (int half = 32; half > 0; half >>= 1) {
+    if (q < half) sums[q][c] += sums[q + half][c];
+    __syncthreads();
   }
+  if (q == 0 && e < D) out[e] = from_f32<T>(sums[0][c]);
 }
 
 // Calls f with the wavefronts a row takes and its steps, as compile-time constants.
@@ -282,11 +321,33 @@ inline void for_width(int64_t D, F f) {
     f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
 }
 
-// Workgroups of the gradient: enough to fill the GPU a few times over, no more than there are rows.
+// The gradient's widths: 8 elements a lane where that is possible, because each element costs a lane
+// five registers (row, gradient, weight, two sums), and the row on its way as much again.
+template <typename F>
+inline void for_grad_width(int64_t D, F f) {
+  using std::integral_constant;
+  if (D <= 512)
+    f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  else if (D <= 1024)
+    f(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+  else if (D <= 1536)
+    f(integral_constant<int, 3>{}, integral_constant<int, 1>{});
+  else if (D <= 2048)
+    f(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  else if (D <= 4096)
+    f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+  else if (D <= 8192)
+    f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else
+    f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+}
+
+// Workgroups of the gradient: what the GPU holds at once (16 wavefronts a CU), no more than there are
+// rows, and no more than 1024, because each leaves two rows of sums for the second kernel.
 int64_t grad_groups(int64_t rows, int64_t D) {
-  const int64_t slots = D <= 2048 ? 4 : 1;
-  const int64_t want = (rows + slots - 1) / slots;
-  return want < 1024 ? want : 1024;
+  const int64_t slots = D <= 512 ? 4 : 1;
+  const int64_t want = (rows + slots - 1) / slots, fit = D <= 2048 ? 1024 : D <= 4096 ? 512 : 256;
+  return want < fit ? want : fit;
 }
 
 bool pieces_ok(int64_t D, std::initializer_list<const void*> ptrs) {
@@ -365,7 +426,7 @@ extern "C" int lema_norm_grad(const void* s, const void* w, const void* gh, cons
   for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     if (rows > 0)
-      for_width(D, [&](auto wc, auto sc) {
+      for_grad_width(D, [&](auto wc, auto sc) {
         constexpr int W = decltype(wc)::value, S = decltype(sc)::value;
         const auto kernel = center ? (vec ? norm_grad_kernel<T, W, S, true, true>
                                           : norm_grad_kernel<T, W, S, false, true>)
@@ -376,7 +437,7 @@ extern "C" int lema_norm_grad(const void* s, const void* w, const void* gh, cons
             static_cast<const T*>(gs), eps, rows, static_cast<int>(D), static_cast<T*>(gx), partial);
       });
     if (sums)
-      norm_weight_kernel<T><<<dim3((D + 15) / 16, gb != nullptr ? 2 : 1), dim3(256), 0, st>>>(
+      norm_weight_kernel<T><<<dim3((D + 15) / 16, gb != nullptr ? 2 : 1), dim3(1024), 0, st>>>(
           partial, static_cast<int>(groups), static_cast<int>(D), static_cast<T*>(gw),
           static_cast<T*>(gb));
   });

@@ -18,7 +18,6 @@ import math
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -64,7 +63,8 @@ def _rows(logits: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
 
 def _check(logits, targets, mask, temperature):
     """The arguments every loss takes, as the kernels read them: (targets, mask)."""
-    _lib.require_device(logits, targets)
+    if not (logits.is_cuda and targets.is_cuda):
+        _lib.require_device(logits, targets)
     if logits.dtype not in _lib.DTYPE_CODE:
         raise TypeError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
     if targets.dtype not in (torch.long, torch.int32):
@@ -77,16 +77,19 @@ def _check(logits, targets, mask, temperature):
         raise ValueError(f"the temperature must be positive, got {temperature}")
     if mask is not None and mask.dtype != torch.bool:
         raise TypeError(f"the mask must be bool, got {mask.dtype}")
-    _lib.same_device(logits, targets=targets, mask=mask)
-    return targets.to(torch.long).contiguous(), _per_token("mask", mask, targets)
+    if targets.device != logits.device or (mask is not None and mask.device != logits.device):
+        _lib.same_device(logits, targets=targets, mask=mask)
+    return targets.long().contiguous(), _per_token("mask", mask, targets)
 
 
 def _per_token(name, t, targets):
     """t, broadcast to the targets' shape, contiguous (None stays None)."""
     if t is None:
         return None
+    if t.shape == targets.shape:
+        return _lib.dense(t)
     try:
-        return t.detach().expand(targets.shape).resolve_neg().contiguous()
+        return _lib.dense(t.expand(targets.shape))
     except RuntimeError:
         raise ValueError(f"{name} {tuple(t.shape)} does not broadcast to the targets "
                          f"{tuple(targets.shape)}") from None
@@ -95,11 +98,15 @@ def _per_token(name, t, targets):
 def _floats(name, t, targets):
     if t is None:
         return None
-    _lib.require_device(t)
-    _lib.same_device(targets, **{name: t})
+    if (t.dtype is torch.float32 and t.shape == targets.shape and t.device == targets.device
+            and t.is_contiguous() and not t.is_neg()):
+        return t
+    if t.device != targets.device:
+        _lib.require_device(t)
+        _lib.same_device(targets, **{name: t})
     if not t.is_floating_point():
         raise TypeError(f"{name} must be floating point, got {t.dtype}")
-    return _per_token(name, t.to(torch.float32), targets)
+    return _per_token(name, t.detach().float(), targets)
 
 
 def _ptr(t):
@@ -112,51 +119,66 @@ def _layout(logits):
     return t, (_lib.DTYPE_CODE[t.dtype], rows, inner, t.shape[-1], so, si)
 
 
-def _grad(ctx, saved, coef, per, scale0, scale1):
-    """The logits' gradient from what the forward saved."""
-    logits, targets, mask, stats = saved
-    dev = coef.device
-    logits = logits.to(device=dev, dtype=ctx.dtype)
-    back = lambda t, dt: None if t is None else _lib.dense(t.to(device=dev, dtype=dt))  # noqa: E731
-    targets, mask, stats = back(targets, torch.long), back(mask, torch.bool), back(stats, torch.float32)
-    t, args = _layout(logits)
-    grad = torch.empty(logits.shape, dtype=t.dtype, device=dev)
-    with _lib.device_of(t):
+# What a forward leaves for its backward is one fp32 tensor: (max, 1 / sum) of each row, then the
+# coefficients (of each row for the policy loss, of each answer for the preference loss), then for
+# the policy loss 1 / the counted rows, and room for the rows' terms.
+
+def _remember(ctx, logits, t, args, targets, mask, state, temperature):
+    ctx.save_for_backward(logits, targets, mask, state)
+    # the description holds for the saved logits unless they were copied to be read
+    ctx.logits = (t.data_ptr(), t.stride(), args) if t is logits else None
+    ctx.dtype, ctx.temperature = logits.dtype, temperature
+    ctx.set_materialize_grads(False)
+
+
+def _grad(ctx, like, coef, per, scale0, inv_n, grad=None):
+    """The logits' gradient from what the forward saved. coef: a tensor, or None for the state's;
+    inv_n: whether the state has it; grad: the one that the forward wrote for scale0 = 1."""
+    logits, targets, mask, state = ctx.saved_tensors
+    dev = like.device
+    if logits.dtype is not ctx.dtype or logits.device != dev:
+        logits = logits.to(device=dev, dtype=ctx.dtype)
+    targets, state = _lib.saved(targets, like, torch.long), _lib.saved(state, like, torch.float32)
+    mask = _lib.saved(mask, like, torch.bool) if mask is not None else None
+    if ctx.logits is not None and ctx.logits[:2] == (logits.data_ptr(), logits.stride()):
+        t, args = logits, ctx.logits[2]
+    else:
+        t, args = _layout(logits)
+    at, rows = state.data_ptr(), args[1]
+    out = grad if grad is not None else torch.empty(logits.shape, dtype=t.dtype, device=dev)
+    with _lib.device_of(like):
         _lib.check(_lib.lib().lema_token_logprobs_grad(
-            t.data_ptr(), *args, targets.data_ptr(), _ptr(mask), ctx.temperature, stats.data_ptr(),
-            coef.data_ptr(), per, _ptr(scale0), _ptr(scale1), grad.data_ptr(), _lib.stream_of(t)))
-    return grad
+            t.data_ptr(), *args, targets.data_ptr(), _ptr(mask), ctx.temperature, at,
+            coef.data_ptr() if coef is not None else at + 8 * rows, per, _ptr(scale0),
+            at + 12 * rows if inv_n else None, grad is not None, out.data_ptr(), _lib.stream_of(like)))
+    return out
 
 
-def _logprobs(logits, targets, mask, temperature, want_stats, want_64=False):
-    """(lp, lp in 64 bits or None, stats or None)."""
-    t, args = _layout(logits)
+def _logprobs(t, args, targets, mask, temperature, stats=None, lp64=None):
     lp = t.new_empty(targets.shape, dtype=torch.float32)
-    lp64 = t.new_empty(targets.shape, dtype=torch.float64) if want_64 else None
-    stats = t.new_empty(targets.shape + (2,), dtype=torch.float32) if want_stats else None
     with _lib.device_of(t):
         _lib.check(_lib.lib().lema_token_logprobs(
             t.data_ptr(), *args, targets.data_ptr(), _ptr(mask), temperature, lp.data_ptr(), _ptr(lp64),
             _ptr(stats), _lib.stream_of(t)))
-    return lp, lp64, stats
-
-
-def _remember(ctx, logits, targets, mask, stats, temperature, *more):
-    ctx.save_for_backward(logits, targets, mask, stats, *more)
-    ctx.dtype, ctx.temperature = logits.dtype, temperature
+    return lp
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, mask, temperature):
-        lp, _, stats = _logprobs(logits, targets, mask, temperature, True)
-        _remember(ctx, logits, targets, mask, stats, temperature)
+        t, args = _layout(logits)
+        state = t.new_empty(2 * args[1], dtype=torch.float32)
+        lp = _logprobs(t, args, targets, mask, temperature, state)
+        _remember(ctx, logits, t, args, targets, mask, state, temperature)
         return lp
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, g):
-        return _grad(ctx, ctx.saved_tensors, _lib.dense(g), 1, None, None), None, None, None
+        if g is None:
+            return (None,) * 4
+        g = _lib.dense(g)
+        return _grad(ctx, g, g, 1, None, False), None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, mask: torch.Tensor | None = None,
@@ -168,34 +190,46 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, mask: torch.Tens
     targets, mask = _check(logits, targets, mask, temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _TokenLogprobs.apply(logits, targets, mask, float(temperature))
-    return _logprobs(logits, targets, mask, float(temperature), False)[0]
+    return _logprobs(*_layout(logits), targets, mask, float(temperature))
 
 
 class _PolicyLoss(torch.autograd.Function):
+    """The forward writes the gradient too, for a gradient of 1 of the loss, while it holds a row's
+    logits: a batch's logits do not fit a cache, and reading them again would be a third of the
+    traffic. The first backward hands that tensor out, computed anew where the loss's gradient
+    is not 1. A second one computes its own, and so does one that is not recorded into the graph
+    that the forward was (its replays would not write the tensor again)."""
+
     @staticmethod
-    def forward(ctx, logits, targets, mask, temperature, old, adv, ref, low, high, kl):
+    def forward(ctx, logits, targets, mask, temperature, old, adv, ref, low, high, kl, want_grad):
         t, args = _layout(logits)
-        f32 = lambda *shape: t.new_empty(shape, dtype=torch.float32)  # noqa: E731
-        lp, stats, loss, inv_n = f32(*targets.shape), f32(*targets.shape, 2), f32(), f32()
-        term, coef = f32(targets.numel()), f32(targets.numel())
+        n = args[1]
+        lp, loss = t.new_empty(targets.shape, dtype=torch.float32), t.new_empty((), dtype=torch.float32)
+        state = t.new_empty(4 * n + 1, dtype=torch.float32)
+        stream = _lib.stream_of(t)
+        at = state.data_ptr()
         with _lib.device_of(t):
+            ctx.capture = _lib.lib().lema_capture_id(stream)
+            ctx.grad = (torch.empty(logits.shape, dtype=t.dtype, device=t.device)
+                        if want_grad and ctx.capture >= 0 else None)
             _lib.check(_lib.lib().lema_policy_loss(
                 t.data_ptr(), *args, targets.data_ptr(), _ptr(mask), temperature, old.data_ptr(),
-                adv.data_ptr(), _ptr(ref), low, high, kl, lp.data_ptr(), stats.data_ptr(),
-                term.data_ptr(), coef.data_ptr(), loss.data_ptr(), inv_n.data_ptr(), _lib.stream_of(t)))
-        _remember(ctx, logits, targets, mask, stats, temperature, coef, inv_n)
+                adv.data_ptr(), _ptr(ref), low, high, kl, lp.data_ptr(), at, at + 12 * n + 4, at + 8 * n,
+                loss.data_ptr(), at + 12 * n, _ptr(ctx.grad), stream))
+        _remember(ctx, logits, t, args, targets, mask, state, temperature)
         ctx.mark_non_differentiable(lp)
-        ctx.set_materialize_grads(False)
         return loss, lp
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, g, _):
         if g is None:
-            return (None,) * 10
-        *saved, coef, inv_n = ctx.saved_tensors
-        coef, inv_n = (_lib.dense(t.to(device=g.device, dtype=torch.float32)) for t in (coef, inv_n))
-        return (_grad(ctx, saved, coef, 1, _lib.dense(g), inv_n),) + (None,) * 9
+            return (None,) * 11
+        g = _lib.dense(g)
+        grad = ctx.__dict__.pop("grad", None)
+        if grad is not None and _lib.lib().lema_capture_id(_lib.stream_of(g)) != ctx.capture:
+            grad = None
+        return (_grad(ctx, g, None, 1, g, True, grad),) + (None,) * 10
 
 
 def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch.Tensor,
@@ -219,34 +253,36 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch
         raise ValueError(f"clip distances must not be negative, got {clip_low} and {clip_high}")
     if kl_weight != 0 and ref is None:
         raise ValueError("kl_weight needs ref_logprobs")
+    want = torch.is_grad_enabled() and logits.requires_grad
     return PolicyLoss(*_PolicyLoss.apply(logits, targets, mask, float(temperature), old, adv, ref,
-                                         float(clip_low), float(clip_high), float(kl_weight)))
+                                         float(clip_low), float(clip_high), float(kl_weight), want))
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, mask, temperature, ref, beta, smooth):
+        t, args = _layout(logits)
         N, T = targets.shape
-        lp, lp64, stats = _logprobs(logits, targets, mask, temperature, True, want_64=True)
-        loss, margins, coef = (lp.new_empty(s) for s in ((), (N // 2,), (N,)))
-        with _lib.device_of(lp):
+        state = t.new_empty(2 * N * T + N, dtype=torch.float32)
+        lp64 = t.new_empty(targets.shape, dtype=torch.float64)
+        lp = _logprobs(t, args, targets, mask, temperature, state, lp64)
+        loss, margins = lp.new_empty(()), lp.new_empty(N // 2)
+        with _lib.device_of(t):
             _lib.check(_lib.lib().lema_preference_loss(
                 lp64.data_ptr(), ref.data_ptr(), _ptr(mask), N // 2, T, beta, smooth, loss.data_ptr(),
-                margins.data_ptr(), coef.data_ptr(), _lib.stream_of(lp)))
-        _remember(ctx, logits, targets, mask, stats, temperature, coef)
+                margins.data_ptr(), state.data_ptr() + 8 * N * T, _lib.stream_of(t)))
+        _remember(ctx, logits, t, args, targets, mask, state, temperature)
+        ctx.per = max(1, T)
         ctx.mark_non_differentiable(margins, lp)
-        ctx.set_materialize_grads(False)
         return loss, margins, lp
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, g, *_):
         if g is None:
             return (None,) * 7
-        *saved, coef = ctx.saved_tensors
-        coef = _lib.dense(coef.to(device=g.device, dtype=torch.float32))
-        T = saved[1].shape[1]
-        return (_grad(ctx, saved, coef, max(1, T), _lib.dense(g), None),) + (None,) * 6
+        g = _lib.dense(g)
+        return (_grad(ctx, g, None, ctx.per, g, False),) + (None,) * 6
 
 
 def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logprobs: torch.Tensor,

@@ -41,7 +41,6 @@ from pathlib import Path
 import torch
 import torch.nn.functional as F
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .attention import code_dtype_for, lema_from_codes, lema_hard, pack_codes
@@ -66,9 +65,8 @@ def _needs_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
-def _saved(t: torch.Tensor, like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """A saved tensor as it was saved: a saved-tensor hook may bring it back in another form."""
-    return _lib.dense(t.to(device=like.device, dtype=dtype))
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
 
 
 def _norm_forward(x, d, w, b, eps, center):
@@ -77,15 +75,14 @@ def _norm_forward(x, d, w, b, eps, center):
     w = w if isinstance(w, torch.Tensor) else None
     h = torch.empty_like(x)
     s = torch.empty_like(x) if d is not None else None
-    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
     with _lib.device_of(x):
         if center:
             _lib.check(_lib.lib().lema_layer_norm(
-                x.data_ptr(), ptr(d), ptr(w), ptr(b), _lib.DTYPE_CODE[x.dtype], eps, x.numel() // D, D,
-                ptr(s), h.data_ptr(), _lib.stream_of(x)))
+                x.data_ptr(), _ptr(d), _ptr(w), _ptr(b), _lib.DTYPE_CODE[x.dtype], eps, x.numel() // D, D,
+                _ptr(s), h.data_ptr(), _lib.stream_of(x)))
         else:
             _lib.check(_lib.lib().lema_rmsnorm_bf16(
-                x.data_ptr(), ptr(d), ptr(w), eps, x.numel() // D, D, ptr(s), h.data_ptr(),
+                x.data_ptr(), _ptr(d), _ptr(w), eps, x.numel() // D, D, _ptr(s), h.data_ptr(),
                 _lib.stream_of(x)))
     return h, s
 
@@ -97,13 +94,14 @@ class _Norm(torch.autograd.Function):
     def forward(ctx, x, d, w, b, D, eps, center):
         h, s = _norm_forward(x, d, w if w is not None else D, b, eps, center)
         ctx.save_for_backward(x if s is None else s, w)
-        ctx.norm = D, eps, center, d is not None, b is not None
+        ctx.norm = D, eps, int(center), d is not None, b is not None
+        ctx.scratch = _lib.lib().lema_norm_grad_workspace_bytes(x.numel() // D, D)
         ctx.w_shape = w.shape if w is not None else b.shape if b is not None else None
         ctx.set_materialize_grads(False)
         return h if s is None else (h, s)
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, gh, gs=None):
         D, eps, center, has_d, has_b = ctx.norm
         want_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
@@ -113,22 +111,19 @@ class _Norm(torch.autograd.Function):
         s, w = ctx.saved_tensors
         gh = _lib.dense(gh)
         gs = _lib.dense(gs) if gs is not None else None
-        s = _saved(s, gh, gh.dtype)
-        w = _saved(w, gh, gh.dtype) if w is not None else None
-        rows = s.numel() // D
-        gx = torch.empty_like(s) if want_x else None
-        gw = gh.new_empty(D) if want_w else None
-        gb = gh.new_empty(D) if want_b and has_b else None
+        s = _lib.saved(s, gh, gh.dtype)
+        w = _lib.saved(w, gh, gh.dtype) if w is not None else None
         L = _lib.lib()
-        n = L.lema_norm_grad_workspace_bytes(rows, D) if want_w or want_b else 0
-        ws = gh.new_empty(n, dtype=torch.uint8)
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        gx = torch.empty_like(s) if want_x else None
+        gw = gh.new_empty(ctx.w_shape) if want_w else None
+        gb = gh.new_empty(ctx.w_shape) if want_b and has_b else None
+        ws = gh.new_empty(ctx.scratch, dtype=torch.uint8) if want_w or want_b else None
         with _lib.device_of(gh):
             _lib.check(L.lema_norm_grad(
-                s.data_ptr(), ptr(w), gh.data_ptr(), ptr(gs), _lib.DTYPE_CODE[s.dtype], int(center), eps,
-                rows, D, ptr(gx), ptr(gw), ptr(gb), ws.data_ptr() if n else None, n, _lib.stream_of(gh)))
-        shape = lambda g: g.view(ctx.w_shape) if g is not None else None  # noqa: E731
-        return gx, gx if has_d else None, shape(gw), shape(gb), None, None, None
+                s.data_ptr(), _ptr(w), gh.data_ptr(), _ptr(gs), _lib.DTYPE_CODE[gh.dtype], center, eps,
+                s.numel() // D, D, _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), ctx.scratch,
+                _lib.stream_of(gh)))
+        return gx, gx if has_d else None, gw, gb, None, None, None
 
 
 def rms_norm(x: torch.Tensor, norm: nn.RMSNorm, d: torch.Tensor | None = None):
@@ -197,21 +192,20 @@ class _Embed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, w, ids, scale, padding):
         ctx.save_for_backward(ids)
-        ctx.table = *w.shape, scale, padding
+        V, D = w.shape
+        ctx.table = V, D, scale, padding, _lib.lib().lema_embedding_grad_workspace_bytes(ids.numel(), V, D)
         return _embed_forward(w, ids, scale)
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, gy):
-        V, D, scale, padding = ctx.table
+        V, D, scale, padding, n = ctx.table
         gy = _lib.dense(gy)
-        ids = _saved(ctx.saved_tensors[0], gy, torch.long)
+        ids = _lib.saved(ctx.saved_tensors[0], gy, torch.long)
         gw = gy.new_empty(V, D)
-        L = _lib.lib()
-        n = L.lema_embedding_grad_workspace_bytes(ids.numel(), V, D)
         ws = gy.new_empty(n, dtype=torch.uint8)
         with _lib.device_of(gy):
-            _lib.check(L.lema_embedding_grad(
+            _lib.check(_lib.lib().lema_embedding_grad(
                 gy.data_ptr(), _lib.DTYPE_CODE[gy.dtype], ids.data_ptr(), ids.numel(), V, D, scale, padding,
                 gw.data_ptr(), ws.data_ptr(), n, _lib.stream_of(gy)))
         return gw, None, None, None
@@ -266,10 +260,10 @@ class _SwiGLUProduct(torch.autograd.Function):
         return _swiglu_forward(g, u)
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, gy):
         gy = _lib.dense(gy)
-        g, u = (_saved(t, gy, gy.dtype) for t in ctx.saved_tensors)
+        g, u = (_lib.saved(t, gy, gy.dtype) for t in ctx.saved_tensors)
         gg, gu = torch.empty_like(g), torch.empty_like(u)
         with _lib.device_of(gy):
             _lib.check(_lib.lib().lema_swiglu_grad_bf16(
@@ -299,10 +293,10 @@ class _CrossEntropySum(torch.autograd.Function):
         return loss.sum()
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, g):
         logits, y, stats = ctx.saved_tensors
-        logits, y, stats = (_saved(t, g, dt) for t, dt in
+        logits, y, stats = (_lib.saved(t, g, dt) for t, dt in
                             ((logits, torch.bfloat16), (y, torch.long), (stats, torch.float32)))
         V = logits.shape[-1]
         rows = logits.numel() // V
@@ -310,7 +304,7 @@ class _CrossEntropySum(torch.autograd.Function):
         with _lib.device_of(g):
             _lib.check(_lib.lib().lema_token_logprobs_grad(
                 logits.data_ptr(), _lib.BF16, rows, max(1, rows), V, 0, V, y.data_ptr(), None, 1.0,
-                stats.data_ptr(), coef.data_ptr(), max(1, rows), None, None, grad.data_ptr(),
+                stats.data_ptr(), coef.data_ptr(), max(1, rows), None, None, 0, grad.data_ptr(),
                 _lib.stream_of(g)))
         return grad, None
 
@@ -357,7 +351,7 @@ class _SkinnyLinear(torch.autograd.Function):
         return _skinny_forward(x, w)
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, gy):
         x, w = ctx.saved_tensors
         g2 = gy.reshape(-1, gy.shape[-1])

@@ -68,7 +68,7 @@ def test_rows_keep_their_bits(dev):
                                    (1024, 1025, 512), (4097, 3001, 513), (16385, 50304, 64),
                                    (65536, 20000, 40), (70001, 131072, 8)])
 def test_gradient(dev, dtype, n, V, D):
-    """Tokens of very different frequencies: lists of none, one, up to 64 and far more rows."""
+    """Tokens of very different frequencies: lists of none, one, up to 32 and far more rows."""
     emb, g = table(dev, V, D, dtype, seed=n)
     u = torch.rand(n, device=dev, generator=g)
     ids = torch.randperm(V, device=dev, generator=g)[((V + 1) ** u).long().clamp_(1, V) - 1]
@@ -79,7 +79,7 @@ def test_gradient(dev, dtype, n, V, D):
     assert torch.equal(gw, again)
 
 
-@pytest.mark.parametrize("n", [63, 64, 65, 95, 96, 97, 128, 5000, 40000])
+@pytest.mark.parametrize("n", [31, 32, 33, 47, 48, 49, 64, 65, 97, 5000, 40000])
 def test_gradient_one_token(dev, n):
     """Every position the same token: lists around the longest that one wavefront adds up."""
     emb, g = table(dev, 9, 72, torch.float32)

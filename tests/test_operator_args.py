@@ -72,12 +72,13 @@ def test_losses(L):
         bad(i, v)
     assert f(None, 2, 0, 1, 8, 0, 8, None, None, 1.0, None, None, None, None) == _lib.OK
     g = L.lema_token_logprobs_grad
-    assert g(P, 2, 4, 4, 8, 0, 8, P, None, 1.0, None, P, 1, None, None, P, None) == _lib.BAD_ARG
-    assert g(P, 2, 4, 4, 8, 0, 8, P, None, 1.0, P, P, 0, None, None, P, None) == _lib.BAD_ARG
+    assert g(P, 2, 4, 4, 8, 0, 8, P, None, 1.0, None, P, 1, None, None, 0, P, None) == _lib.BAD_ARG
+    assert g(P, 2, 4, 4, 8, 0, 8, P, None, 1.0, P, P, 0, None, None, 0, P, None) == _lib.BAD_ARG
+    assert g(P, 2, 4, 4, 8, 0, 8, P, None, 1.0, P, P, 1, None, None, 1, P, None) == _lib.BAD_ARG
     p = L.lema_policy_loss
-    args = [P, 2, 4, 4, 8, 0, 8, P, None, 1.0, P, P, None, 0.2, 0.2, 0.0, P, P, P, P, P, P, None]
+    args = [P, 2, 4, 4, 8, 0, 8, P, None, 1.0, P, P, None, 0.2, 0.2, 0.0, P, P, P, P, P, P, None, None]
     for i, v in ((10, None), (11, None), (13, -0.1), (14, float("nan")), (16, None), (17, None), (17, P + 4),
-                 (18, None), (19, None), (20, None), (21, None)):
+                 (18, None), (19, None), (20, None), (21, None), (22, P + 1)):
         a = list(args)
         a[i] = v
         assert p(*a) == _lib.BAD_ARG, (i, v)
