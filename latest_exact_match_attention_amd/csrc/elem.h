@@ -40,6 +40,22 @@ union Piece {
   T e[kPiece<T>];
 };
 
+// 16 bytes from or to memory, past the caches where kStream is set.
+template <bool kStream>
+__device__ __forceinline__ u32x4 get16(const void* p) {
+  const u32x4* at = static_cast<const u32x4*>(p);
+  if constexpr (kStream) return __builtin_nontemporal_load(at);
+  return *at;
+}
+template <bool kStream>
+__device__ __forceinline__ void put16(void* p, u32x4 v) {
+  u32x4* at = static_cast<u32x4*>(p);
+  if constexpr (kStream)
+    __builtin_nontemporal_store(v, at);
+  else
+    *at = v;
+}
+
 // Calls f(T{}) with the element type of `dtype` (checked by the caller).
 template <typename F>
 inline void for_dtype(int32_t dtype, F f) {

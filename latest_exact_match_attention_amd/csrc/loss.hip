@@ -36,7 +36,7 @@ struct Scale {
     lo = static_cast<float>(k2 - hi);
   }
   __device__ __forceinline__ float exp(float d) const {
-    return __builtin_amdgcn_exp2f(fmaf(d, lo, d * hi));
+    return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo));
   }
 };
 
@@ -114,14 +114,6 @@ __device__ __forceinline__ int64_t head_of(const T* row, int64_t V) {
 // took 468 us, not 496.
 constexpr int64_t kStreamBytes = int64_t(256) << 20;
 
-template <bool kStream>
-__device__ __forceinline__ void put(u32x4* at, u32x4 v) {
-  if constexpr (kStream)
-    __builtin_nontemporal_store(v, at);
-  else
-    *at = v;
-}
-
 // A row of zeros: `head` elements, 16-byte pieces, `rest` elements from `tail` on.
 template <typename T, int kThreads, bool kStream>
 __device__ __forceinline__ void write_zeros(T* g, int64_t head, int64_t tail, int64_t rest, int64_t pieces) {
@@ -130,14 +122,14 @@ __device__ __forceinline__ void write_zeros(T* g, int64_t head, int64_t tail, in
   if (tid < head) g[tid] = zero;
   if (tid < rest) g[tail + tid] = zero;
   u32x4* out = reinterpret_cast<u32x4*>(g + head);
-  for (int64_t p = tid; p < pieces; p += kThreads) put<kStream>(out + p, u32x4{0, 0, 0, 0});
+  for (int64_t p = tid; p < pieces; p += kThreads) put16<kStream>(out + p, u32x4{0, 0, 0, 0});
 }
 
 // One workgroup per row.
 template <typename T, int kThreads>
 __global__ __launch_bounds__(kThreads) void logprob_kernel(const T* logits, Rows rows, int64_t V,
                                                            const int64_t* target, const uint8_t* mask,
-                                                           float k, Scale k2, float* lp_out, double* lp64_out,
+                                                           float temperature, Scale k2, float* lp_out, double* lp64_out,
                                                            float2* stats, Policy pol) {
   constexpr int kWaves = kThreads / 64, n = kPiece<T>;
   __shared__ Running part[kWaves];
@@ -197,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const T* logits, Rows
   for (int w = 1; w < kWaves; ++w) r = join(r, part[w], k2);
   const int64_t t = target[row];
   const float xt = t >= 0 && t < V ? to_f32(x[t]) : NAN;
-  const double lp = static_cast<double>(xt - r.m) * k - log(static_cast<double>(r.s));
+  const double lp = (static_cast<double>(xt) - r.m) / temperature - log(static_cast<double>(r.s));
   lp_out[row] = static_cast<float>(lp);
   if (lp64_out != nullptr) lp64_out[row] = lp;
   if (stats != nullptr) stats[row] = make_float2(r.m, 1.0f / r.s);
@@ -323,7 +315,7 @@ __global__ __launch_bounds__(kThreads, P > 7 ? 4 : 8) void policy_grad_kernel(
           for (int i = 0; i < n; ++i)
             if (i == body_t % n) o.e[i] = from_f32<T>(hit(to_f32(q[u].e[i])));
         }
-        put<kStream>(out + p, o.raw);
+        put16<kStream>(out + p, o.raw);
       }
     }
   };
@@ -509,7 +501,7 @@ __global__ __launch_bounds__(kThreads) void logprob_grad_kernel(
         if (p >= pieces) break;
 #pragma unroll
         for (int i = 0; i < n; ++i) q[u].e[i] = one(head + p * n + i, to_f32(q[u].e[i]));
-        put<kStream>(out + p, q[u].raw);
+        put16<kStream>(out + p, q[u].raw);
       }
     }
   }
@@ -543,7 +535,7 @@ int logprob_launch(const void* logits, int32_t dtype, int64_t rows, int64_t inne
     const bool wide = wide_rows(dtype, V);
     const auto kernel = wide ? logprob_kernel<T, 1024> : logprob_kernel<T, 256>;
     kernel<<<dim3(rows), dim3(wide ? 1024 : 256), 0, st>>>(
-        static_cast<const T*>(logits), Rows{inner, so, si}, V, target, mask, 1.0f / temperature,
+        static_cast<const T*>(logits), Rows{inner, so, si}, V, target, mask, temperature,
         Scale(temperature), lp, lp64, reinterpret_cast<float2*>(stats), pol);
   });
   return launch_status("logprob_kernel");

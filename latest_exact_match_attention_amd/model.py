@@ -139,6 +139,7 @@ def rms_norm(x: torch.Tensor, norm: nn.RMSNorm, d: torch.Tensor | None = None):
 
 
 def _norm(x, d, w, b, D, eps, center):
+    """norm(x + d) and x + d of contiguous inputs that the kernels take, with or without a graph."""
     if _needs_grad(x, d, w, b):
         out = _Norm.apply(x, d, w, b, D, eps, center)
         return out if d is not None else (out, x)
@@ -160,19 +161,20 @@ def layer_norm(x: torch.Tensor, norm: nn.LayerNorm, d: torch.Tensor | None = Non
     if not x.is_cuda or x.dtype not in _lib.DTYPE_CODE:
         x = x if d is None else x + d
         return norm(x), x
-    dims = tuple(norm.normalized_shape)
-    if tuple(x.shape[x.dim() - len(dims):]) != dims:
-        raise ValueError(f"x {tuple(x.shape)} does not end in the norm's shape {dims}")
+    dims, shape = norm.normalized_shape, x.shape
+    if shape[len(shape) - len(dims):] != dims:
+        raise ValueError(f"x {tuple(shape)} does not end in the norm's shape {tuple(dims)}")
     D = math.prod(dims)
     if not 1 <= D <= LAYER_NORM_MAX:
         raise ValueError(f"rows of {D} elements: layer_norm takes 1 to {LAYER_NORM_MAX}")
     w, b = norm.weight, norm.bias
-    _lib.same_device(x, d=d, weight=w, bias=b)
     for name, t in (("the addend", d), ("the weight", w), ("the bias", b)):
-        if t is not None and t.dtype != x.dtype:
+        if t is not None and (t.dtype is not x.dtype or t.device != x.device):
+            _lib.same_device(x, **{name: t})
             raise TypeError(f"{name} is {t.dtype}, x is {x.dtype}")
     s = x
-    x, d, w, b = (None if t is None else _lib.dense(t) for t in (x, d, w, b))
+    x, w, b = _lib.dense(x), None if w is None else _lib.dense(w), None if b is None else _lib.dense(b)
+    d = None if d is None else _lib.dense(d)
     h, r = _norm(x, d, w, b, D, float(norm.eps), True)
     return h, s if d is None else r
 
@@ -227,7 +229,7 @@ def embed(emb: nn.Embedding, ids: torch.Tensor, scale: float = 1.0) -> torch.Ten
             and not (grad and (emb.sparse or emb.scale_grad_by_freq or w.shape[0] > 1 << 20))):
         y = emb(ids)
         return y if scale == 1.0 else y * scale
-    ids = ids.to(torch.long).contiguous()
+    ids = ids.long().contiguous()
     if grad:
         return _Embed.apply(w, ids, float(scale), -1 if emb.padding_idx is None else emb.padding_idx)
     return _embed_forward(w, ids, float(scale))

@@ -79,7 +79,7 @@ def test_gradient(dev, dtype, n, V, D):
     assert torch.equal(gw, again)
 
 
-@pytest.mark.parametrize("n", [31, 32, 33, 47, 48, 49, 64, 65, 97, 5000, 40000])
+@pytest.mark.parametrize("n", [31, 32, 33, 63, 64, 65, 97, 127, 128, 200, 5000, 40000])
 def test_gradient_one_token(dev, n):
     """Every position the same token: lists around the longest that one wavefront adds up."""
     emb, g = table(dev, 9, 72, torch.float32)
