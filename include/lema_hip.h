@@ -311,15 +311,15 @@ int lema_token_logprobs_grad(const void* logits, int32_t dtype, int64_t rows, in
  *   term = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
  *          + kl (e^(ref_lp - lp) - (ref_lp - lp) - 1)        (ref_lp NULL or kl 0: without)
  *   coef = d term / d lp;  both 0 for rows that the mask leaves out
- * loss = mean of the counted rows' terms (0 without any), inv_n = 1 / counted rows: the gradient
- * of the loss is lema_token_logprobs_grad with coef, per = 1 and inv_n as a scale.
+ * loss = scale * mean of the counted rows' terms (0 without any), inv_n = scale / counted rows: the
+ * gradient of the loss is lema_token_logprobs_grad with coef, per = 1 and inv_n as a scale.
  *   grad  NULL, or contiguous [rows, V] of `dtype` that receives that gradient for a gradient of
  *         1 of the loss: rows of up to 256 KB that start on the same bytes of a 16-byte piece as
  *         grad's are then read once for both */
 int lema_policy_loss(const void* logits, int32_t dtype, int64_t rows, int64_t inner, int64_t V,
                      int64_t so, int64_t si, const int64_t* target, const uint8_t* mask,
                      float temperature, const float* old_lp, const float* advantage,
-                     const float* ref_lp, float clip_low, float clip_high, float kl, float* lp,
+                     const float* ref_lp, float clip_low, float clip_high, float kl, float scale, float* lp,
                      float* stats, float* term, float* coef, float* loss, float* inv_n, void* grad,
                      void* stream);
 

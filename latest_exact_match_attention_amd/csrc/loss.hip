@@ -332,9 +332,10 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
-// inv_n = 1 / counted rows (1 where there are none). 16 mask bytes a thread at a time where they are
+// inv_n = scale / counted rows (scale where there are none). 16 mask bytes a thread at a time where they are
 // aligned to it.
-__global__ __launch_bounds__(1024) void policy_count_kernel(const uint8_t* mask, int64_t rows, float* inv_n) {
+__global__ __launch_bounds__(1024) void policy_count_kernel(const uint8_t* mask, int64_t rows, float scale,
+                                                            float* inv_n) {
   __shared__ uint32_t sums[16];
   uint32_t n = 0;
   const bool pieces = (reinterpret_cast<uintptr_t>(mask) & 15) == 0;
@@ -358,7 +359,7 @@ __global__ __launch_bounds__(1024) void policy_count_kernel(const uint8_t* mask,
   __syncthreads();
   if (threadIdx.x != 0) return;
   for (int w = 1; w < 16; ++w) n += sums[w];
-  *inv_n = n > 0 ? static_cast<float>(1.0 / n) : 1.0f;
+  *inv_n = n > 0 ? static_cast<float>(scale / static_cast<double>(n)) : scale;
 }
 
 // loss = sum of the terms * inv_n, in 64 bits; `term` starts at a 4-byte boundary of any kind.
@@ -615,7 +616,7 @@ extern "C" int lema_policy_loss(const void* logits, int32_t dtype, int64_t rows,
                                 int64_t so, int64_t si, const int64_t* target, const uint8_t* mask,
                                 float temperature, const float* old_lp, const float* advantage,
                                 const float* ref_lp, float clip_low, float clip_high, float kl,
-                                float* lp, float* stats, float* term, float* coef, float* loss,
+                                float scale, float* lp, float* stats, float* term, float* coef, float* loss,
                                 float* inv_n, void* grad, void* stream) {
   clear_error();
   if (int rc = check_logits(logits, dtype, rows, inner, V, so, si, target, temperature)) return rc;
@@ -627,7 +628,7 @@ extern "C" int lema_policy_loss(const void* logits, int32_t dtype, int64_t rows,
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Policy pol{old_lp, advantage, kl != 0.0f ? ref_lp : nullptr, term, coef, clip_low, clip_high, kl};
   const bool fused = grad != nullptr && rows > 0 && one_pass(logits, grad, dtype, rows, inner, V, so, si);
-  policy_count_kernel<<<dim3(1), dim3(1024), 0, st>>>(mask, rows, inv_n);
+  policy_count_kernel<<<dim3(1), dim3(1024), 0, st>>>(mask, rows, scale, inv_n);
   if (fused) {
     for_dtype(dtype, [&](auto t) {
       using T = decltype(t);

@@ -201,7 +201,7 @@ class _PolicyLoss(torch.autograd.Function):
     that the forward was (its replays would not write the tensor again)."""
 
     @staticmethod
-    def forward(ctx, logits, targets, mask, temperature, old, adv, ref, low, high, kl, want_grad):
+    def forward(ctx, logits, targets, mask, temperature, old, adv, ref, low, high, kl, scale, want_grad):
         t, args = _layout(logits)
         n = args[1]
         lp, loss = t.new_empty(targets.shape, dtype=torch.float32), t.new_empty((), dtype=torch.float32)
@@ -214,7 +214,7 @@ class _PolicyLoss(torch.autograd.Function):
                         if want_grad and ctx.capture >= 0 else None)
             _lib.check(_lib.lib().lema_policy_loss(
                 t.data_ptr(), *args, targets.data_ptr(), _ptr(mask), temperature, old.data_ptr(),
-                adv.data_ptr(), _ptr(ref), low, high, kl, lp.data_ptr(), at, at + 12 * n + 4, at + 8 * n,
+                adv.data_ptr(), _ptr(ref), low, high, kl, scale, lp.data_ptr(), at, at + 12 * n + 4, at + 8 * n,
                 loss.data_ptr(), at + 12 * n, _ptr(ctx.grad), stream))
         _remember(ctx, logits, t, args, targets, mask, state, temperature)
         ctx.mark_non_differentiable(lp)
@@ -224,25 +224,29 @@ class _PolicyLoss(torch.autograd.Function):
     @_lib.once
     def backward(ctx, g, _):
         if g is None:
-            return (None,) * 11
+            return (None,) * 12
         g = _lib.dense(g)
         grad = ctx.__dict__.pop("grad", None)
         if grad is not None and _lib.lib().lema_capture_id(_lib.stream_of(g)) != ctx.capture:
             grad = None
-        return (_grad(ctx, g, None, 1, g, True, grad),) + (None,) * 10
+        return (_grad(ctx, g, None, 1, g, True, grad),) + (None,) * 11
 
 
 def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch.Tensor,
                 advantages: torch.Tensor, ref_logprobs: torch.Tensor | None = None,
                 mask: torch.Tensor | None = None, clip_low: float = 0.2, clip_high: float = 0.2,
-                kl_weight: float = 0.0, temperature: float = 1.0) -> PolicyLoss:
-    """The mean over the counted positions of
+                kl_weight: float = 0.0, temperature: float = 1.0, scale: float = 1.0) -> PolicyLoss:
+    """`scale` times the mean over the counted positions of
 
         -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_weight (e^g - g - 1)
 
     with lp = token_logprobs(logits, targets), r = e^(lp - old_logprobs), A = advantages and
     g = ref_logprobs - lp; 0 where the mask counts nothing. old_logprobs, advantages, ref_logprobs
-    and mask broadcast to the targets' shape ([B, 1] advantages give each answer one)."""
+    and mask broadcast to the targets' shape ([B, 1] advantages give each answer one).
+
+    The forward already writes the logits' gradient for a gradient of 1 of the loss. A factor that
+    the loss is to have (one over the steps that gradients are accumulated for) is best given as
+    `scale`: multiplied afterwards, it makes the backward read the logits again."""
     targets, mask = _check(logits, targets, mask, temperature)
     old, adv, ref = (_floats(n, t, targets) for n, t in
                      (("old_logprobs", old_logprobs), ("advantages", advantages),
@@ -251,11 +255,13 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch
         raise TypeError("old_logprobs and advantages are needed")
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError(f"clip distances must not be negative, got {clip_low} and {clip_high}")
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be a number, got {scale}")
     if kl_weight != 0 and ref is None:
         raise ValueError("kl_weight needs ref_logprobs")
     want = torch.is_grad_enabled() and logits.requires_grad
     return PolicyLoss(*_PolicyLoss.apply(logits, targets, mask, float(temperature), old, adv, ref,
-                                         float(clip_low), float(clip_high), float(kl_weight), want))
+                                         float(clip_low), float(clip_high), float(kl_weight), float(scale), want))
 
 
 class _PreferenceLoss(torch.autograd.Function):

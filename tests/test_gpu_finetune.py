@@ -169,3 +169,92 @@ def test_swiglu_gradient(dev):
     for got, want, size in ((ga, y * u * sig * (1 + x * (1 - sig)), (y * u * sig).abs() * (1 + x.abs())),
                             (gb, y * x * sig, (y * x * sig).abs())):
         assert bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 16 * 2.0 ** -24 * size + 1e-38).all())
+
+
+def operators(dev, seed):
+    """A call of each operator with its gradients, on inputs of its own: () -> list of tensors."""
+    from latest_exact_match_attention_amd.model import embed, layer_norm
+    g = torch.Generator(dev).manual_seed(seed)
+    emb = torch.nn.Embedding(3000, 264, device=dev, dtype=torch.bfloat16)
+    norm = torch.nn.LayerNorm(264, device=dev, dtype=torch.bfloat16)
+    head = (torch.randn(1003, 264, device=dev, generator=g) * 0.06).bfloat16().requires_grad_(True)
+    ids = torch.randint(0, 3000, (8, 200), device=dev, generator=g)
+    targets = torch.randint(0, 1003, (8, 200), device=dev, generator=g)
+    adv = torch.randn(8, 1, device=dev, generator=g)
+    old = torch.full((8, 200), -6.9, device=dev)
+    with torch.no_grad():
+        emb.weight.copy_(torch.randn(3000, 264, device=dev, generator=g))
+
+    def run():
+        h, _ = layer_norm(embed(emb, ids, 2.0), norm)
+        logits = h @ head.t()
+        loss = policy_loss(logits, targets, old, adv, old, kl_weight=0.1).loss \
+            + preference_loss(logits, targets, old).loss + token_logprobs(logits, targets).mean()
+        return [loss.detach(), *torch.autograd.grad(loss, [emb.weight, norm.weight, norm.bias, head])]
+    return run
+
+
+def test_streams_at_once(dev):
+    """Two callers on streams of their own, their launches interleaved: the results of each alone."""
+    runs = [operators(dev, s) for s in (1, 2)]
+    want = [r() for r in runs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in runs]
+    got = [[], []]
+    for _ in range(6):
+        for k, (r, s) in enumerate(zip(runs, streams)):
+            with torch.cuda.stream(s):
+                got[k].append(r())
+    torch.cuda.synchronize()
+    for k in range(2):
+        for out in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
+
+
+def test_offsets_beyond_32_bits(dev):
+    """Rows, tables and logits of more than 2^31 elements: what lies at their ends."""
+    from latest_exact_match_attention_amd.model import embed, layer_norm
+    V, D = 1_000_000, 2200
+    emb = torch.nn.Embedding(V, D, _weight=torch.zeros(V, D, device=dev, dtype=torch.bfloat16))
+    with torch.no_grad():
+        emb.weight[-3:] = 1.5
+    ids = torch.tensor([V - 1, 0, V - 1, V - 3, V - 5], device=dev)
+    y = embed(emb, ids)
+    assert y[:, 0].tolist() == [1.5, 0.0, 1.5, 1.5, 0.0]
+    (gw,) = torch.autograd.grad(y, [emb.weight], torch.ones_like(y))
+    assert gw[[0, 1, V - 5, V - 4, V - 3, V - 2, V - 1]].float().mean(1).tolist() == [1, 0, 1, 0, 1, 0, 2]
+    del emb, y, gw
+    R, D = 270_000, 8000
+    norm = torch.nn.LayerNorm(D, device=dev, dtype=torch.bfloat16)
+    x = torch.zeros(R, D, device=dev, dtype=torch.bfloat16)
+    x[-2:] = torch.randn(2, D, device=dev).bfloat16()
+    x.requires_grad_(True)
+    h, _ = layer_norm(x, norm)
+    gh = torch.zeros_like(h)
+    gh[-2:] = torch.randn(2, D, device=dev).bfloat16()
+    gx, gw = torch.autograd.grad(h, [x, norm.weight], gh)
+    t = x.detach()[-2:].clone().requires_grad_(True)
+    h2, _ = layer_norm(t, norm)
+    gt, gw2 = torch.autograd.grad(h2, [t, norm.weight], gh[-2:])
+    assert torch.equal(h[-2:], h2) and torch.equal(gx[-2:], gt) and not gx[:-2:1000].any()
+    assert torch.allclose(gw.float(), gw2.float(), rtol=2 ** -7, atol=0)    # one rounding of bf16 each
+    del x, h, gh, gx
+    n, V = 43_000, 50_304
+    logits = torch.zeros(n, V, device=dev, dtype=torch.bfloat16)
+    logits[-1] = torch.randn(V, device=dev).bfloat16()
+    logits.requires_grad_(True)
+    targets = torch.full((n,), 17, device=dev)
+    mask = torch.zeros(n, dtype=torch.bool, device=dev)
+    mask[-1] = True
+    z = torch.full((n,), -9.0, device=dev)
+    r = policy_loss(logits, targets, z, z, mask=mask, clip_low=1.0, clip_high=1e9)
+    (g,) = torch.autograd.grad(r.loss, [logits])
+    one = logits.detach()[-1:].clone().requires_grad_(True)
+    s = policy_loss(one, targets[-1:], z[-1:], z[-1:], clip_low=1.0, clip_high=1e9)
+    (w,) = torch.autograd.grad(s.loss, [one])
+    assert torch.equal(r.loss, s.loss) and torch.equal(g[-1:], w) and not g[:-1:997].any()
+    lp = token_logprobs(logits, targets, mask)
+    (g,) = torch.autograd.grad(lp.sum(), [logits])
+    one_lp = token_logprobs(one, targets[-1:])
+    (w,) = torch.autograd.grad(one_lp.sum(), [one])
+    assert torch.equal(lp[-1:], one_lp) and torch.equal(g[-1:], w)

@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from latest_exact_match_attention_amd import _lib
 from latest_exact_match_attention_amd.loss import policy_loss, preference_loss, token_logprobs
 from latest_exact_match_attention_amd.model import cross_entropy_sum
 
@@ -206,9 +207,36 @@ def test_policy_temperature_broadcast_and_scale(dev):
         old = token_logprobs(logits, targets, temperature=1.3) - 0.05
     adv = torch.randn(4, 1, device=dev)
     r = policy_loss(logits, targets, old, adv, mask=mask[:, :1], temperature=1.3)
-    (grad,) = torch.autograd.grad(-2.5 * r.loss, [logits])
-    check_policy(r, grad, logits.detach(), targets, old, adv.expand(4, 33), ref, mask[:, :1].expand(4, 33),
-                 0.2, 0.2, 0.0, 1.3, -2.5)
+    # the gradient is computed anew where the loss's is not 1, and by every backward but the first
+    (a,) = torch.autograd.grad(r.loss, [logits], retain_graph=True)
+    (grad,) = torch.autograd.grad(-2.5 * r.loss, [logits], retain_graph=True)
+    (b,) = torch.autograd.grad(r.loss, [logits])
+    args = (logits.detach(), targets, old, adv.expand(4, 33), ref, mask[:, :1].expand(4, 33), 0.2, 0.2, 0.0, 1.3)
+    for g, up in ((a, 1.0), (grad, -2.5), (b, 1.0)):
+        check_policy(r, g, *args, up)
+    s = policy_loss(logits, targets, old, adv, mask=mask[:, :1], temperature=1.3, scale=0.25)
+    assert abs(float(s.loss.detach()) - 0.25 * float(r.loss.detach())) <= 4 * E * abs(float(r.loss.detach()))
+    (grad,) = torch.autograd.grad(s.loss, [logits])
+    check_policy(r, grad, *args, 0.25)
+
+
+def test_policy_backward_in_another_graph(dev, monkeypatch):
+    """A backward that is recorded into another graph than the forward (or into one, where the
+    forward was not) writes a tensor of its own, whatever the loss's gradient: a replay finds no
+    forward before it."""
+    logits, targets, old, adv, ref, mask = policy_case(dev, (2, 30), 1000, torch.float32)
+    logits.requires_grad_(True)
+    first = []
+    empty = torch.empty
+    with monkeypatch.context() as m:
+        m.setattr(torch, "empty", lambda *a, **k: first.append(empty(*a, **k)) or first[-1])
+        r = policy_loss(logits, targets, old, adv, mask=mask)
+    assert [t.shape for t in first] == [logits.shape]        # the forward's gradient
+    first[0].fill_(7.0)
+    monkeypatch.setattr(_lib.lib(), "lema_capture_id", lambda stream: 5)
+    (g,) = torch.autograd.grad(r.loss, [logits])
+    assert g.data_ptr() != first[0].data_ptr() and bool((first[0] == 7.0).all())
+    check_policy(r, g, logits.detach(), targets, old, adv, ref, mask, 0.2, 0.2, 0.0)
 
 
 def test_masked_rows_are_not_read(dev):

@@ -76,9 +76,9 @@ def test_losses(L):
     assert g(P, 2, 4, 4, 8, 0, 8, P, None, 1.0, P, P, 0, None, None, 0, P, None) == _lib.BAD_ARG
     assert g(P, 2, 4, 4, 8, 0, 8, P, None, 1.0, P, P, 1, None, None, 1, P, None) == _lib.BAD_ARG
     p = L.lema_policy_loss
-    args = [P, 2, 4, 4, 8, 0, 8, P, None, 1.0, P, P, None, 0.2, 0.2, 0.0, P, P, P, P, P, P, None, None]
-    for i, v in ((10, None), (11, None), (13, -0.1), (14, float("nan")), (16, None), (17, None), (17, P + 4),
-                 (18, None), (19, None), (20, None), (21, None), (22, P + 1)):
+    args = [P, 2, 4, 4, 8, 0, 8, P, None, 1.0, P, P, None, 0.2, 0.2, 0.0, 1.0, P, P, P, P, P, P, None, None]
+    for i, v in ((10, None), (11, None), (13, -0.1), (14, float("nan")), (17, None), (18, None), (18, P + 4),
+                 (19, None), (20, None), (21, None), (22, None), (23, P + 1)):
         a = list(args)
         a[i] = v
         assert p(*a) == _lib.BAD_ARG, (i, v)
