@@ -259,7 +259,8 @@ int lema_embedding(const void* table, int32_t dtype, int64_t vocab, int64_t D, c
  * do not occur and for token `padding` (negative: none). Ids outside [0, vocab) take no part.
  *   gy   contiguous [n, D] of `dtype`; n < 2^31 - 16384, vocab and D at most 2^20
  *   workspace  256-byte aligned, lema_embedding_grad_workspace_bytes(n, vocab, D) bytes: about
- *              16 bytes a position, 4 a token, and n / 64 rows of fp32 */
+ *              16 bytes a position, 4 a token, and n / 64 rows of fp32 (n / 16 up to 16384
+ *              positions), padded to 512 */
 int64_t lema_embedding_grad_workspace_bytes(int64_t n, int64_t vocab, int64_t D);
 int lema_embedding_grad(const void* gy, int32_t dtype, const int64_t* ids, int64_t n, int64_t vocab,
                         int64_t D, float scale, int64_t padding, void* gw, void* workspace,

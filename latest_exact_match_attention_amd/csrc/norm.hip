@@ -22,12 +22,12 @@ namespace {
 
 constexpr int64_t kMaxD = 16384;
 
-// Where lane `lane` of a row's W wavefronts finds its 8 elements of step s: next to each other in
-// 16-byte pieces (kVec), or 64 * W apart, so that a wavefront's loads of single elements
-// are contiguous too.
-template <int W, bool kVec>
+// Where lane `lane` of a row's W wavefronts finds its element k of step s: in 16-byte pieces, a load's
+// pieces next to each other (kVec), or single elements, a load's next to each other.
+template <typename T, int W, bool kVec>
 __device__ __forceinline__ int elem_at(int s, int k, int lane) {
-  return kVec ? (s * W * 64 + lane) * 8 + k : (s * 8 + k) * W * 64 + lane;
+  constexpr int n = kVec ? kPiece<T> : 1;
+  return ((s * 8 + k) / n * W * 64 + lane) * n + k % n;
 }
 
 // A row's elements as they come from memory, so that a row can be on its way while the one before
@@ -42,15 +42,15 @@ struct RawRow {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       if constexpr (kVec) {
-        const int e = elem_at<W, true>(s, 0, lane);
 #pragma unroll
-        for (int i = 0; i < 8 / n; ++i)
-          q[s * 8 / n + i].raw =
-              e < D ? get16<kStream>(p + e + i * n) : u32x4{0, 0, 0, 0};
+        for (int i = 0; i < 8 / n; ++i) {
+          const int e = elem_at<T, W, true>(s, i * n, lane);
+          q[s * 8 / n + i].raw = e < D ? get16<kStream>(p + e) : u32x4{0, 0, 0, 0};
+        }
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int e = elem_at<W, false>(s, k, lane);
+          const int e = elem_at<T, W, false>(s, k, lane);
           q[(s * 8 + k) / n].e[k % n] = e < D ? p[e] : T{};
         }
       }
@@ -72,19 +72,21 @@ __device__ __forceinline__ void store_row(T* p, int D, int lane, const float (&v
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     if constexpr (kVec) {
-      const int e = elem_at<W, true>(s, 0, lane);
       constexpr int n = kPiece<T>;
-      if (e < D) {
-        Piece<T> q[8 / n];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) q[k / n].e[k % n] = from_f32<T>(v[s * 8 + k]);
+      for (int i = 0; i < 8 / n; ++i) {
+        const int e = elem_at<T, W, true>(s, i * n, lane);
+        if (e < D) {
+          Piece<T> q;
 #pragma unroll
-        for (int i = 0; i < 8 / n; ++i) put16<kStream>(p + e + i * n, q[i].raw);
+          for (int k = 0; k < n; ++k) q.e[k] = from_f32<T>(v[s * 8 + i * n + k]);
+          put16<kStream>(p + e, q.raw);
+        }
       }
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int e = elem_at<W, false>(s, k, lane);
+        const int e = elem_at<T, W, false>(s, k, lane);
         if (e < D) p[e] = from_f32<T>(v[s * 8 + k]);
       }
     }
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(64 * group_waves(W)) void layer_norm_kernel(
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       v[s * 8 + k] -= m;
-      if (elem_at<W, kVec>(s, k, lane) < D) sum[0] += v[s * 8 + k] * v[s * 8 + k];
+      if (elem_at<T, W, kVec>(s, k, lane) < D) sum[0] += v[s * 8 + k] * v[s * 8 + k];
     }
   row_sums<W, 1>(sum, red, turn);
   const float r = rsqrtf(sum[0] / static_cast<float>(D) + eps);
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
       for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          v[s * 8 + k] = elem_at<W, kVec>(s, k, lane) < D ? v[s * 8 + k] - m : 0.0f;
+          v[s * 8 + k] = elem_at<T, W, kVec>(s, k, lane) < D ? v[s * 8 + k] - m : 0.0f;
     }
     float sum[3] = {0.0f, 0.0f, 0.0f};  // of squares, of a v, of a
 #pragma unroll
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
       for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int e = elem_at<W, kVec>(s, k, lane);
+          const int e = elem_at<T, W, kVec>(s, k, lane);
           comb[slot * 512 * S + e] = which ? gb[s * 8 + k] : gw[s * 8 + k];
         }
       __syncthreads();
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
       for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int e = elem_at<W, kVec>(s, k, lane);
+          const int e = elem_at<T, W, kVec>(s, k, lane);
           if (e < D) out[e] = which ? gb[s * 8 + k] : gw[s * 8 + k];
         }
     }
