@@ -543,9 +543,13 @@ int embed_launch(const void* table, int32_t dtype, int64_t vocab, int64_t D, con
     // many rows go past the Infinity Cache, and leave it to the table's frequent ones: 65,536 of 1536
     // in bf16 took 40 us, not 60
     const bool past = n * D * static_cast<int64_t>(sizeof(T)) > (int64_t(128) << 20);
-    const auto kernel = !vec   ? (scaled ? embed_kernel<T, false, true, false> : embed_kernel<T, false, false, false>)
-                        : past ? (scaled ? embed_kernel<T, true, true, true> : embed_kernel<T, true, false, true>)
-                               : (scaled ? embed_kernel<T, true, true, false> : embed_kernel<T, true, false, false>);
+    const auto pick = [&](auto scales) {
+      constexpr bool kScale = decltype(scales)::value;
+      return !vec   ? embed_kernel<T, false, kScale, false>
+             : past ? embed_kernel<T, true, kScale, true>
+                    : embed_kernel<T, true, kScale, false>;
+    };
+    const auto kernel = scaled ? pick(std::true_type{}) : pick(std::false_type{});
     kernel<<<dim3(grid), dim3(256), 0, st>>>(static_cast<const T*>(table), vocab, D, ids, n,
                                              static_cast<int>(slices), scale, static_cast<T*>(out));
   });

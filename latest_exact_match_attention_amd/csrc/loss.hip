@@ -75,7 +75,8 @@ __device__ __forceinline__ float policy_row(const Policy& pol, int64_t row, floa
 }
 
 struct Running {
-  float m, s;  // the maximum so far, -FLT_MAX at least, and the sum rescaled to it
+  float m;   // the maximum so far, -FLT_MAX at least
+  double s;  // the sum rescaled to it: 64 bits, so that a likely token's 1 does not round the others off
 };
 
 // Adds n logits to r. -FLT_MAX for the maximum of nothing, or of -inf alone, keeps
@@ -89,13 +90,18 @@ __device__ __forceinline__ void add_logits(Running& r, const float (&x)[N], Scal
     r.s *= k2.exp(r.m - bm);
     r.m = bm;
   }
-  float sa = 0.0f, sb = 0.0f;
+  constexpr int kLines = N < 8 ? N : 8;  // short lines of additions, for the same reason
+  float e[kLines];
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    sa += k2.exp(x[i] - r.m);
-    if (i + 1 < N) sb += k2.exp(x[i + 1] - r.m);
+  for (int i = 0; i < N; ++i) {
+    const float v = k2.exp(x[i] - r.m);
+    e[i % kLines] = i < kLines ? v : e[i % kLines] + v;
   }
-  r.s += sa + sb;
+#pragma unroll
+  for (int d = kLines / 2; d > 0; d /= 2)
+#pragma unroll
+    for (int i = 0; i < d; ++i) e[i] += e[i + d];
+  r.s += e[0];
 }
 
 __device__ __forceinline__ Running join(Running a, Running b, Scale k2) {
@@ -129,8 +135,8 @@ __device__ __forceinline__ void write_zeros(T* g, int64_t head, int64_t tail, in
 template <typename T, int kThreads>
 __global__ __launch_bounds__(kThreads) void logprob_kernel(const T* logits, Rows rows, int64_t V,
                                                            const int64_t* target, const uint8_t* mask,
-                                                           float temperature, Scale k2, float* lp_out, double* lp64_out,
-                                                           float2* stats, Policy pol) {
+                                                           float temperature, Scale k2, float* lp_out,
+                                                           double* lp64_out, float2* stats, Policy pol) {
   constexpr int kWaves = kThreads / 64, n = kPiece<T>;
   __shared__ Running part[kWaves];
   const int64_t row = blockIdx.x;
@@ -146,7 +152,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const T* logits, Rows
   const T* x = logits + rows.at(row);
   const int64_t head = head_of(x, V), pieces = (V - head) / n, tail = head + pieces * n;
   const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
-  Running r{-FLT_MAX, 0.0f};
+  Running r{-FLT_MAX, 0.0};
   if (tid < head) {  // head < n <= 8 elements
     const float one[1] = {to_f32(x[tid])};
     add_logits<1>(r, one, k2);
@@ -189,10 +195,10 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const T* logits, Rows
   for (int w = 1; w < kWaves; ++w) r = join(r, part[w], k2);
   const int64_t t = target[row];
   const float xt = t >= 0 && t < V ? to_f32(x[t]) : NAN;
-  const double lp = (static_cast<double>(xt) - r.m) / temperature - log(static_cast<double>(r.s));
+  const double lp = (static_cast<double>(xt) - r.m) / temperature - log(r.s);
   lp_out[row] = static_cast<float>(lp);
   if (lp64_out != nullptr) lp64_out[row] = lp;
-  if (stats != nullptr) stats[row] = make_float2(r.m, 1.0f / r.s);
+  if (stats != nullptr) stats[row] = make_float2(r.m, static_cast<float>(1.0 / r.s));
   if (pol.old != nullptr)
     policy_row(pol, row, static_cast<float>(lp), pol.old[row], pol.adv[row],
                pol.ref != nullptr ? pol.ref[row] : 0.0f);
@@ -319,9 +325,9 @@ __global__ __launch_bounds__(kThreads, P > 7 ? 4 : 8) void policy_grad_kernel(
       }
     }
   };
-  if (fabsf(mk) < 1e37f)
+  if (fabsf(mk) < 1048576.0f)  // its rounding is then below 2^-4
     finish([&](float v) { return __builtin_amdgcn_exp2f(fmaf(v, k2.hi, -mk)); }, fmaf(m, k2.hi, -mk));
-  else  // the product leaves fp32's range, the differences need not
+  else  // logits of any size, up to those whose product leaves fp32's range
     finish([&](float v) { return __builtin_amdgcn_exp2f((v - m) * k2.hi); }, 0.0f);
 }
 
@@ -332,8 +338,8 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
-// inv_n = scale / counted rows (scale where there are none). 16 mask bytes a thread at a time where they are
-// aligned to it.
+// inv_n = scale / counted rows (scale where there are none). 16 mask bytes a thread at a time where
+// they are aligned to it.
 __global__ __launch_bounds__(1024) void policy_count_kernel(const uint8_t* mask, int64_t rows, float scale,
                                                             float* inv_n) {
   __shared__ uint32_t sums[16];

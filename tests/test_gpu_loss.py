@@ -119,32 +119,34 @@ def test_values_at_the_edge(dev):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [12, 1001, 50304, 131073])
 def test_policy_values_at_the_edge(dev, dtype, V):
-    """Rows whose maximum times log2 e leaves fp32's range, rows of -inf with one logit, and a NaN:
-    the loss and its gradient from the kernel that holds a row (and, at the last size, from the
+    """Rows whose maximum times log2 e leaves fp32's range or is large in it, rows of -inf with one
+    logit, and a NaN: the loss and its gradient from the kernel that holds a row (and, at the last size, from the
     ones that do not)."""
     top = torch.finfo(dtype).max
-    x = torch.zeros(5, V, device=dev, dtype=dtype)
+    x = torch.zeros(6, V, device=dev, dtype=dtype)
+    big = {torch.float32: 2.0 ** 30, torch.float16: 2.0 ** 15, torch.bfloat16: 2.0 ** 100}[dtype]
+    x[5], x[5, 2:] = big, -big
     x[0] = -top
     x[1, 1:], x[1, 0] = -top, top
     x[2], x[2, 3] = -float("inf"), 1.0
     x[3, 7] = float("nan")
     x[4, ::2] = -float("inf")
-    t = torch.tensor([5, 0, 3, 1, 1], device=dev)
-    z, one = torch.zeros(5, device=dev), torch.ones(5, device=dev)
+    t = torch.tensor([5, 0, 3, 1, 1, 1], device=dev)
+    z, one = torch.zeros(6, device=dev), torch.ones(6, device=dev)
     x.requires_grad_(True)
-    for rows in ([0, 1, 2, 4], [3]):
-        mask = torch.zeros(5, dtype=torch.bool, device=dev)
+    for rows in ([0, 1, 2, 4, 5], [3]):
+        mask = torch.zeros(6, dtype=torch.bool, device=dev)
         mask[rows] = True
         r = policy_loss(x, t, torch.where(t == 5, -math.log(V), 0.0), one, mask=mask, clip_high=1e3)
         (g,) = torch.autograd.grad(r.loss, [x])
         if rows == [3]:
             assert bool(r.loss.isnan() and r.logprobs[3].isnan() and g[3].isnan().all())
-            assert not g[[0, 1, 2, 4]].any()
+            assert not g[[0, 1, 2, 4, 5]].any()
             continue
         want = torch.log_softmax(x.detach().double(), -1)
         lp = want.gather(1, t[:, None])[:, 0]
         assert bool(((r.logprobs - lp).abs()[rows] <= 128 * E * lp.abs().clamp_min(1)[rows]).all())
-        c = -torch.exp(lp - torch.where(t == 5, -math.log(V), 0.0)).double()[:, None] / 4
+        c = -torch.exp(lp - torch.where(t == 5, -math.log(V), 0.0)).double()[:, None] / 5
         exact_g = c * (torch.nn.functional.one_hot(t, V) - want.exp())
         u = torch.finfo(dtype).eps / 2
         assert bool(((g.double() - exact_g).abs() <= u * exact_g.abs() + 256 * E * c.abs() + 2.0 ** -25)[rows].all())
