@@ -203,6 +203,15 @@ def saved(t: torch.Tensor, like: torch.Tensor, dtype: torch.dtype) -> torch.Tens
     return dense(t.to(device=like.device, dtype=dtype))
 
 
+def needs_grad(*ts) -> bool:
+    """Whether autograd wants to know of an operation on the tensors (None is passed over): one of
+    them asks for its gradient, or forward mode is on, which a Function without it refuses where a
+    kernel's output would silently be a constant. The level has no public name."""
+    if getattr(torch.autograd.forward_ad, "_current_level", -1) >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
 def once(backward):
     """A Function's backward whose gradients have none themselves, as torch's once_differentiable
     does it, but at no cost (that takes 6 us) where nobody records them."""

@@ -188,7 +188,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, mask: torch.Tens
     answer, and of the reference. One read of the logits, and one more read and a write for
     their gradient."""
     targets, mask = _check(logits, targets, mask, temperature)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _lib.needs_grad(logits):
         return _TokenLogprobs.apply(logits, targets, mask, float(temperature))
     return _logprobs(*_layout(logits), targets, mask, float(temperature))
 

@@ -60,11 +60,6 @@ def _fused(*ts: torch.Tensor) -> bool:
     return True
 
 
-def _needs_grad(*ts) -> bool:
-    """Whether autograd wants a gradient of one of the tensors (None is passed over)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
-
-
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
@@ -140,7 +135,7 @@ def rms_norm(x: torch.Tensor, norm: nn.RMSNorm, d: torch.Tensor | None = None):
 
 def _norm(x, d, w, b, D, eps, center):
     """norm(x + d) and x + d of contiguous inputs that the kernels take, with or without a graph."""
-    if _needs_grad(x, d, w, b):
+    if _lib.needs_grad(x, d, w, b):
         out = _Norm.apply(x, d, w, b, D, eps, center)
         return out if d is not None else (out, x)
     h, s = _norm_forward(x, d, w if w is not None else D, b, eps, center)
@@ -222,7 +217,7 @@ def embed(emb: nn.Embedding, ids: torch.Tensor, scale: float = 1.0) -> torch.Ten
     sparse gradient or one scaled by frequency, a table of more than 2^20 rows that wants a
     gradient, and CPU tensors take the torch operations."""
     w = emb.weight
-    grad = _needs_grad(w)
+    grad = _lib.needs_grad(w)
     if not (w.is_cuda and ids.device == w.device and w.dtype in _lib.DTYPE_CODE and w.is_contiguous()
             and ids.dtype in (torch.long, torch.int32) and emb.max_norm is None and w.numel()
             and w.shape[1] <= 1 << 20
@@ -277,7 +272,7 @@ class _SwiGLUProduct(torch.autograd.Function):
 def swiglu(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
     if not (_fused(g, u) and g.numel() % 8 == 0):
         return F.silu(g) * u
-    return _SwiGLUProduct.apply(g, u) if _needs_grad(g, u) else _swiglu_forward(g, u)
+    return _SwiGLUProduct.apply(g, u) if _lib.needs_grad(g, u) else _swiglu_forward(g, u)
 
 
 class _CrossEntropySum(torch.autograd.Function):
@@ -318,7 +313,7 @@ def cross_entropy_sum(logits: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
         return F.cross_entropy(logits.float(), y, reduction="sum")
     rows = logits.numel() // V
     yy = y.reshape(-1).to(torch.int64).contiguous()
-    if _needs_grad(logits):
+    if _lib.needs_grad(logits):
         return _CrossEntropySum.apply(logits, yy)
     loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
     _lib.check(_lib.lib().lema_cross_entropy_bf16(
@@ -366,7 +361,7 @@ def linear(x: torch.Tensor, lin: nn.Linear) -> torch.Tensor:
     """lin(x); a decode-shaped product (<= 32 rows, bf16) on the skinny MFMA kernel."""
     if not _skinny(x, lin.weight):
         return lin(x)
-    if _needs_grad(x, lin.weight):
+    if _lib.needs_grad(x, lin.weight):
         return _SkinnyLinear.apply(x, lin.weight)
     return _skinny_forward(x, lin.weight)
 
@@ -538,7 +533,7 @@ class SwiGLU(nn.Module):
         accumulates into `residual` itself, which is then returned."""
         g, u, dn = self.gate.weight, self.up.weight, self.down.weight
         if _skinny(x, g) and g.shape == u.shape and u.data_ptr() % 16 == 0 and u.is_contiguous() \
-                and not _needs_grad(x, g, u, dn, residual):
+                and not _lib.needs_grad(x, g, u, dn, residual):
             K, N = x.shape[-1], g.shape[0]
             M = x.numel() // K
             a = x.new_empty(x.shape[:-1] + (N,))
@@ -767,7 +762,7 @@ class Transformer(nn.Module):
 
     def _embed(self, idx):
         """The token rows: `embed`, whose gradient sorts the tokens, where one is wanted."""
-        return embed(self.tok_emb, idx) if _needs_grad(self.tok_emb.weight) else self.tok_emb(idx)
+        return embed(self.tok_emb, idx) if _lib.needs_grad(self.tok_emb.weight) else self.tok_emb(idx)
 
     def hidden(self, idx):
         """The final normalised hidden states (the input of lm_head), without a cache."""

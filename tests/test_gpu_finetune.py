@@ -258,3 +258,20 @@ def test_offsets_beyond_32_bits(dev):
     one_lp = token_logprobs(one, targets[-1:])
     (w,) = torch.autograd.grad(one_lp.sum(), [one])
     assert torch.equal(lp[-1:], one_lp) and torch.equal(g[-1:], w)
+
+
+def test_forward_mode_is_refused(dev):
+    """A tangent is never dropped: the operators have no forward mode and say so."""
+    import torch.autograd.forward_ad as fwd
+    from latest_exact_match_attention_amd.model import layer_norm, rms_norm
+    x = torch.randn(4, 64, device=dev).bfloat16()
+    t = torch.zeros(4, dtype=torch.long, device=dev)
+    z = torch.zeros(4, device=dev)
+    norm, rms = (n(64, device=dev, dtype=torch.bfloat16) for n in (torch.nn.LayerNorm, torch.nn.RMSNorm))
+    with torch.no_grad(), fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: layer_norm(d, norm), lambda: rms_norm(d, rms), lambda: swiglu(d, d),
+                     lambda: token_logprobs(d, t), lambda: policy_loss(d, t, z, z),
+                     lambda: preference_loss(d[:, None], t[:, None], z[:, None])):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
