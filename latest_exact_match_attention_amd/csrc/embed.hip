@@ -303,8 +303,12 @@ __global__ __launch_bounds__(512) void embed_order_kernel(Order o) {
   };
   for (int k = t; k < 8 * rows; k += 512) cursors[k] = 0;
   __syncthreads();
+  // counted a digit at a time: 64 lanes of one frequent token would queue for its word
   each([&](uint32_t i0, uint32_t id, uint32_t) {
-    if (i0 + lane < end) atomicAdd(&cur[id & (rows - 1)], 1u);
+    const bool live = i0 + lane < end;
+    const uint64_t m = same_digit(id & (rows - 1), o.row_bits, __ballot(live));
+    if (live && (m & ((uint64_t(1) << lane) - 1)) == 0) cur[id & (rows - 1)] += __popcll(m);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   });
   __syncthreads();
   uint32_t mine[2] = {0, 0};  // tokens 2 t and 2 t + 1 of the bucket
