@@ -31,12 +31,21 @@ def check_grad(gw, ids, gy, V, scale, padding=None):
     if padding is not None:
         keep &= ids != padding
     ids, gy = ids[keep], gy[keep]
-    want, size, m = (torch.zeros(V, n, dtype=torch.float64, device=gw.device) for n in (D, D, 1))
-    want.index_add_(0, ids, gy * scale)
-    size.index_add_(0, ids, gy.abs() * abs(scale))
-    m.index_add_(0, ids, torch.ones_like(gy[:, :1]))
+    # running sums of the rows in the tokens' order (index_add_ in 64 bits takes minutes where
+    # millions of positions hold one token: they wait for each other at its row)
+    order = torch.argsort(ids, stable=True)
+    m = torch.bincount(ids, minlength=V)[:, None]
+    ends = m.cumsum(0)[:, 0]
+
+    def sums(rows):
+        run = torch.zeros(rows.shape[0] + 1, D, dtype=torch.float64, device=gw.device)
+        torch.cumsum(rows[order], 0, out=run[1:])
+        return run[ends] - run[ends - m[:, 0]]
+    want, size = sums(gy * scale), sums(gy.abs() * abs(scale))
     u, tiny = half_step(gw.dtype)
     tol = u * want.abs() + (m + 3) * 2.0 ** -24 * size + tiny * (m > 0)
+    # the running sums themselves are off by less than 2^-50 of all the rows' sum
+    tol = tol + 2.0 ** -50 * gy.abs().sum() * abs(scale) / max(1, D)
     assert bool(((gw.double() - want).abs() <= tol).all())
 
 
@@ -77,6 +86,23 @@ def test_gradient(dev, dtype, n, V, D):
     check_grad(gw, ids, gy, V, 1.5)
     (again,) = torch.autograd.grad(embed(emb, ids, 1.5), [emb.weight], gy)
     assert torch.equal(gw, again)
+
+
+@pytest.mark.parametrize("dtype,n,V,D", [(torch.bfloat16, 3000, 700, 2048), (torch.float32, 2500, 40, 4096),
+                                         (torch.float16, 20000, 90, 1541), (torch.bfloat16, 3000, 1 << 20, 8),
+                                         (torch.float32, 900, (1 << 20) + 1, 8),
+                                         (torch.bfloat16, 1_200_000, 50304, 8),
+                                         (torch.float16, 17_000_001, 3000, 8)])
+def test_gradient_of_the_largest(dev, dtype, n, V, D):
+    """Rows of more slices than a wavefront takes, the largest table (and one past it, which
+    nn.Embedding's own gradient takes), and more positions than 64 and than 1024 spans hold."""
+    emb, g = table(dev, V, D, dtype, seed=n)
+    u = torch.rand(n, device=dev, generator=g, dtype=torch.float64)
+    ids = ((V + 1) ** u).long().clamp_(1, V) - 1
+    ids[-1] = V - 1
+    gy = torch.randn(n, D, device=dev, generator=g).to(dtype)
+    (gw,) = torch.autograd.grad(embed(emb, ids), [emb.weight], gy)
+    check_grad(gw, ids, gy, V, 1.0)
 
 
 @pytest.mark.parametrize("n", [31, 32, 33, 63, 64, 65, 97, 127, 128, 200, 5000, 40000])
