@@ -244,13 +244,12 @@ int lema_embedding_bf16(const void* table, int64_t vocab, int64_t D, const int64
                         int64_t n, void* out, void* stream);
 
 /* ---- a training step around the exact op: embedding, norms and losses with gradients ----
- * All three value types. The reference trains these with torch's own operations
- * (code/lema/model.py, code/lema/train.py); the policy and preference losses have no
- * counterpart there. Work on the same workspace or outputs must be ordered by the caller. */
+ * All three value types; tensors of values may start at any element. The reference trains these
+ * with torch's own operations (code/lema/model.py, code/lema/train.py); the policy and preference
+ * losses have no counterpart there. Work on the same workspace or outputs must be ordered by the caller. */
 
 /* out row i = table row ids[i] * scale, rounded once (the bits as they are where scale is 1),
- * zeros for an id outside [0, vocab). table contiguous [vocab, D], 1 <= D <= 2^20, aligned to an
- * element; rows of D % 8 == 0 on 16-byte boundaries are read in 16-byte pieces. */
+ * zeros for an id outside [0, vocab). table contiguous [vocab, D], 1 <= D <= 2^20. */
 int lema_embedding(const void* table, int32_t dtype, int64_t vocab, int64_t D, const int64_t* ids,
                    int64_t n, float scale, void* out, void* stream);
 
@@ -315,8 +314,7 @@ int lema_token_logprobs_grad(const void* logits, int32_t dtype, int64_t rows, in
  * loss = scale * mean of the counted rows' terms (0 without any), inv_n = scale / counted rows: the
  * gradient of the loss is lema_token_logprobs_grad with coef, per = 1 and inv_n as a scale.
  *   grad  NULL, or contiguous [rows, V] of `dtype` that receives that gradient for a gradient of
- *         1 of the loss: rows of up to 256 KB that start on the same bytes of a 16-byte piece as
- *         grad's are then read once for both */
+ *         1 of the loss: rows of up to 256 KB are then read once for both */
 int lema_policy_loss(const void* logits, int32_t dtype, int64_t rows, int64_t inner, int64_t V,
                      int64_t so, int64_t si, const int64_t* target, const uint8_t* mask,
                      float temperature, const float* old_lp, const float* advantage,

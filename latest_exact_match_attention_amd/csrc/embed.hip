@@ -31,70 +31,36 @@ __device__ __forceinline__ int wave_index() {
   return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
 }
 
-// C slices of 512 columns of a row, as they come from memory.
-template <typename T, int C, bool kVec>
-struct RawSlices {
-  Piece<T> q[C * 8 / kPiece<T>];
-
+// C slices of 512 columns of a row, as they come from memory, a load's units next to each other.
+template <typename T, int C, int kKind>
+struct RawSlices : RowPart<T, kKind, C * 8> {
+  typedef RowPart<T, kKind, C * 8> Part;
+  static __device__ __forceinline__ auto columns(int64_t c0, int lane) {
+    return [=](int i) { return c0 + i * 64 + lane * kUnit<T, kKind>; };
+  }
   template <bool kStream = false>
   __device__ __forceinline__ void fetch(const T* row, int64_t c0, int64_t D, int lane) {
-    constexpr int n = kPiece<T>;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      if constexpr (kVec) {
-#pragma unroll
-        for (int i = 0; i < 8 / n; ++i) {  // a load's pieces next to each other
-          const int64_t e = c0 + c * kCols + (i * 64 + lane) * n;
-          q[c * 8 / n + i].raw = e < D ? get16<kStream>(row + e) : u32x4{0, 0, 0, 0};
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int64_t e = c0 + c * kCols + k * 64 + lane;
-          q[(c * 8 + k) / n].e[k % n] = e < D ? row[e] : T{};
-        }
-      }
-    }
+    Part::template fetch<kStream>(row, D, columns(c0, lane));
   }
+  __device__ __forceinline__ void settle(int64_t c0, int64_t D, int lane) { Part::settle(D, columns(c0, lane)); }
   template <bool kStream>
   __device__ __forceinline__ void store(T* row, int64_t c0, int64_t D, int lane) const {
-    constexpr int n = kPiece<T>;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      if constexpr (kVec) {
-#pragma unroll
-        for (int i = 0; i < 8 / n; ++i) {
-          const int64_t e = c0 + c * kCols + (i * 64 + lane) * n;
-          if (e < D) put16<kStream>(row + e, q[c * 8 / n + i].raw);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int64_t e = c0 + c * kCols + k * 64 + lane;
-          if (e < D) row[e] = q[(c * 8 + k) / n].e[k % n];
-        }
-      }
-    }
+    Part::template store<kStream>(row, D, columns(c0, lane));
   }
-  __device__ __forceinline__ float at(int k) const { return to_f32(q[k / kPiece<T>].e[k % kPiece<T>]); }
-  __device__ __forceinline__ void set(int k, float v) { q[k / kPiece<T>].e[k % kPiece<T>] = from_f32<T>(v); }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int k = 0; k < C * 8 / kPiece<T>; ++k) q[k].raw = u32x4{0, 0, 0, 0};
-  }
+  __device__ __forceinline__ float at(int k) const { return this->get(k); }
 };
 
 // fp32 sums of C slices as a row's elements.
-template <typename T, int C, bool kVec, bool kStream>
+template <typename T, int C, int kKind, bool kStream>
 __device__ __forceinline__ void store_slices(T* row, int64_t c0, int64_t D, int lane, const float (&v)[C * 8]) {
-  RawSlices<T, C, kVec> r;
+  RawSlices<T, C, kKind> r;
 #pragma unroll
   for (int k = 0; k < C * 8; ++k) r.set(k, v[k]);
   r.template store<kStream>(row, c0, D, lane);
 }
 
 // One wavefront per (position, 512 columns).
-template <typename T, bool kVec, bool kScale, bool kStream>
+template <typename T, int kKind, bool kScale, bool kStream>
 __global__ __launch_bounds__(256) void embed_kernel(const T* table, int64_t vocab, int64_t D,
                                                     const int64_t* ids, int64_t n, int slices,
                                                     float scale, T* out) {
@@ -104,8 +70,9 @@ __global__ __launch_bounds__(256) void embed_kernel(const T* table, int64_t voca
   if (i >= n) return;
   const int64_t c0 = (u - i * slices) * kCols, id = ids[i];
   const bool ok = id >= 0 && id < vocab;
-  RawSlices<T, 1, kVec> r;
+  RawSlices<T, 1, kKind> r;
   r.fetch(table + (ok ? id : 0) * D, c0, D, lane);
+  r.settle(c0, D, lane);
   if constexpr (kScale) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) r.set(k, r.at(k) * scale);
@@ -348,7 +315,7 @@ __global__ __launch_bounds__(512) void embed_order_kernel(Order o) {
 }
 
 // acc += gy rows perm[j], j in [j0, j1), in order: 64 positions read at once, 4 or 8 rows in flight.
-template <typename T, int C, bool kVec, bool kStream>
+template <typename T, int C, int kKind, bool kStream>
 __device__ __forceinline__ void add_rows(const T* gy, const uint32_t* perm, uint32_t j0, uint32_t j1,
                                          int64_t c0, int64_t D, int lane, float (&acc)[C * 8]) {
   for (uint32_t j = j0; j < j1; j += 64) {
@@ -356,7 +323,7 @@ __device__ __forceinline__ void add_rows(const T* gy, const uint32_t* perm, uint
     const uint32_t pos = perm[j + min(lane, m - 1)];
     constexpr int kRows = C == 1 ? 8 : 4;
     for (int i = 0; i < m; i += kRows) {
-      RawSlices<T, C, kVec> v[kRows];
+      RawSlices<T, C, kKind> v[kRows];
 #pragma unroll
       for (int u = 0; u < kRows; ++u) {
         const uint32_t p = __builtin_amdgcn_readlane(pos, min(i + u, m - 1));
@@ -365,6 +332,7 @@ __device__ __forceinline__ void add_rows(const T* gy, const uint32_t* perm, uint
 #pragma unroll
       for (int u = 0; u < kRows; ++u)
         if (u == 0 || i + u < m) {
+          v[u].settle(c0, D, lane);
 #pragma unroll
           for (int k = 0; k < C * 8; ++k) acc[k] += v[u].at(k);
         }
@@ -377,7 +345,7 @@ __host__ __device__ inline int64_t padded_cols(int64_t D) { return (D + kCols - 
 
 // One wavefront per (tile or token, C slices of 512 columns): the tiles come first. partial: [tiles,
 // padded_cols(D)].
-template <typename T, int C, bool kVec, bool kStream>
+template <typename T, int C, int kKind, bool kStream>
 __global__ __launch_bounds__(256) void embed_sum_kernel(Order o, const T* gy, int64_t D, int slices,
                                                         int64_t tiles, float scale, float* partial,
                                                         T* gw) {
@@ -393,7 +361,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(Order o, const T* gy, in
     if (j0 + o.tile > o.start[o.vocab]) return;
     const uint32_t v = o.token[j0];
     if (o.token[j0 + o.tile - 1] != v || o.start[v + 1] - o.start[v] <= kLong) return;
-    add_rows<T, C, kVec, kStream>(gy, o.perm, j0, j0 + o.tile, c0, D, lane, acc);
+    add_rows<T, C, kKind, kStream>(gy, o.perm, j0, j0 + o.tile, c0, D, lane, acc);
 #pragma unroll
     for (int c = 0; c < C; ++c)
       if (c0 + c * kCols < D) {
@@ -412,10 +380,10 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(Order o, const T* gy, in
     const int64_t v = item - tiles;
     const uint32_t j0 = o.start[v], j1 = o.start[v + 1];
     if (j1 - j0 > kLong) return;
-    add_rows<T, C, kVec, kStream>(gy, o.perm, j0, j1, c0, D, lane, acc);
+    add_rows<T, C, kKind, kStream>(gy, o.perm, j0, j1, c0, D, lane, acc);
 #pragma unroll
     for (int k = 0; k < C * 8; ++k) acc[k] *= scale;
-    store_slices<T, C, kVec, kStream>(gw + v * D, c0, D, lane, acc);
+    store_slices<T, C, kKind, kStream>(gw + v * D, c0, D, lane, acc);
   }
 }
 
@@ -423,7 +391,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(Order o, const T* gy, in
 // sums and the positions after the last one, each dealt out to the 16 wavefronts, the tiles 4 at a time
 // in flight: the most frequent token of 65,536 has about 120. 64 registers, so that a CU holds two
 // workgroups.
-template <typename T, bool kVec, bool kStream>
+template <typename T, int kKind, bool kStream>
 __global__ __launch_bounds__(1024, 8) void embed_join_kernel(Order o, const T* gy, int64_t D, float scale,
                                                           const float* partial, T* gw) {
   __shared__ float sums[16][8][64];
@@ -441,8 +409,9 @@ __global__ __launch_bounds__(1024, 8) void embed_join_kernel(Order o, const T* g
     for (uint32_t i = 0; i < 2 * tile; i += 16) {
       const uint32_t at = (i < tile ? j0 : tail) + (i & (tile - 1)) + w;
       if (at < (i < tile ? head : j1)) {
-        RawSlices<T, 1, kVec> r;
+        RawSlices<T, 1, kKind> r;
         r.template fetch<kStream>(gy + static_cast<int64_t>(o.perm[at]) * D, c0, D, lane);
+        r.settle(c0, D, lane);
 #pragma unroll
         for (int k = 0; k < 8; ++k) acc[k] += r.at(k);
       }
@@ -480,7 +449,7 @@ __global__ __launch_bounds__(1024, 8) void embed_join_kernel(Order o, const T* g
     if (w == 0) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) acc[k] = sums[0][k][lane];
-      store_slices<T, 1, kVec, kStream>(gw + v * D, c0, D, lane, acc);
+      store_slices<T, 1, kKind, kStream>(gw + v * D, c0, D, lane, acc);
     }
     __syncthreads();
   }
@@ -541,21 +510,23 @@ int embed_launch(const void* table, int32_t dtype, int64_t vocab, int64_t D, con
                  int64_t n, float scale, void* out, hipStream_t st) {
   const int64_t slices = (D + kCols - 1) / kCols, grid = (n * slices + 3) / 4;
   LEMA_REQUIRE(grid < (int64_t(1) << 31), "too many ids");
-  const bool vec = D % 8 == 0 && aligned(table, 16) && aligned(out, 16), scaled = scale != 1.0f;
+  const RowKind kind = row_kind(dtype, D);
+  // many rows go past the Infinity Cache, and leave it to the table's frequent ones: 65,536 of 1536 in
+  // bf16 took 40 us, not 60
+  const bool past = kind == kWholeRows && aligned(out, 16) && n * D * dtype_size(dtype) > (int64_t(128) << 20);
   for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    // many rows go past the Infinity Cache, and leave it to the table's frequent ones: 65,536 of 1536
-    // in bf16 took 40 us, not 60
-    const bool past = n * D * static_cast<int64_t>(sizeof(T)) > (int64_t(128) << 20);
-    const auto pick = [&](auto scales) {
-      constexpr bool kScale = decltype(scales)::value;
-      return !vec   ? embed_kernel<T, false, kScale, false>
-             : past ? embed_kernel<T, true, kScale, true>
-                    : embed_kernel<T, true, kScale, false>;
+    const auto launch = [&](auto kernel) {
+      kernel<<<dim3(grid), dim3(256), 0, st>>>(static_cast<const T*>(table), vocab, D, ids, n,
+                                               static_cast<int>(slices), scale, static_cast<T*>(out));
     };
-    const auto kernel = scaled ? pick(std::true_type{}) : pick(std::false_type{});
-    kernel<<<dim3(grid), dim3(256), 0, st>>>(static_cast<const T*>(table), vocab, D, ids, n,
-                                             static_cast<int>(slices), scale, static_cast<T*>(out));
+    if (past)
+      launch(scale != 1.0f ? embed_kernel<T, kWholeRows, true, true> : embed_kernel<T, kWholeRows, false, true>);
+    else
+      for_kind<T>(kind, [&](auto k) {
+        constexpr int kKind = decltype(k)::value;
+        launch(scale != 1.0f ? embed_kernel<T, kKind, true, false> : embed_kernel<T, kKind, false, false>);
+      });
   });
   return launch_status("embed_kernel");
 }
@@ -614,31 +585,30 @@ extern "C" int lema_embedding_grad(const void* gy, int32_t dtype, const int64_t*
   if (o.spans > 1) embed_count_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
   embed_scatter_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
   embed_order_kernel<<<dim3(o.buckets), dim3(512), 8 * 4 << o.row_bits, st>>>(o);
-  const bool vec = D % 8 == 0 && aligned(gy, 16) && aligned(gw, 16);
+  const RowKind kind = row_kind(dtype, D);
+  // rows in, and the table's gradient out, past the Infinity Cache where they are larger than it: 65,536
+  // rows of 1536 and a table of 50,304 in bf16 took 71 us, not 85
+  const bool past = kind == kWholeRows && aligned(gy, 16) && aligned(gw, 16) &&
+                    (n + vocab) * D * size > (int64_t(256) << 20);
   for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    // rows in, and the table's gradient out, past the Infinity Cache where they are larger than it:
-    // 65,536 rows of 1536 and a table of 50,304 in bf16 took 71 us, not 85
-    const bool past = (n + vocab) * D * size > (int64_t(256) << 20);
-    const auto pick = [&](auto c) {
-      constexpr int C = decltype(c)::value;
-      return !vec   ? embed_sum_kernel<T, C, false, false>
-             : past ? embed_sum_kernel<T, C, true, true>
-                    : embed_sum_kernel<T, C, true, false>;
-    };
-    const auto sum = per == 1   ? pick(std::integral_constant<int, 1>{})
-                     : per == 2 ? pick(std::integral_constant<int, 2>{})
-                                : pick(std::integral_constant<int, 3>{});
-    sum<<<dim3(grid), dim3(256), 0, st>>>(o, static_cast<const T*>(gy), D, static_cast<int>(slices),
-                                          tiles, scale, partial, static_cast<T*>(gw));
-    if (longest > 0) {
-      const auto join = !vec   ? embed_join_kernel<T, false, false>
-                        : past ? embed_join_kernel<T, true, true>
-                               : embed_join_kernel<T, true, false>;
+    const auto run = [&](auto k, auto stream) {
+      constexpr int kKind = decltype(k)::value;
+      constexpr bool kStream = decltype(stream)::value;
+      const auto sum = per == 1   ? embed_sum_kernel<T, 1, kKind, kStream>
+                       : per == 2 ? embed_sum_kernel<T, 2, kKind, kStream>
+                                  : embed_sum_kernel<T, 3, kKind, kStream>;
+      sum<<<dim3(grid), dim3(256), 0, st>>>(o, static_cast<const T*>(gy), D, static_cast<int>(slices),
+                                            tiles, scale, partial, static_cast<T*>(gw));
       const int64_t at_once = longest < 256 ? longest : 256;
-      join<<<dim3(at_once, cols), dim3(1024), 0, st>>>(o, static_cast<const T*>(gy), D, scale, partial,
-                                                       static_cast<T*>(gw));
-    }
+      if (longest > 0)
+        embed_join_kernel<T, kKind, kStream><<<dim3(at_once, cols), dim3(1024), 0, st>>>(
+            o, static_cast<const T*>(gy), D, scale, partial, static_cast<T*>(gw));
+    };
+    if (past)
+      run(std::integral_constant<int, kWholeRows>{}, std::true_type{});
+    else
+      for_kind<T>(kind, [&](auto k) { run(k, std::false_type{}); });
   });
   return launch_status("the embedding gradient's kernels");
 }

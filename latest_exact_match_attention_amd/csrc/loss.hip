@@ -127,8 +127,7 @@ __device__ __forceinline__ void write_zeros(T* g, int64_t head, int64_t tail, in
   const T zero = from_f32<T>(0.0f);
   if (tid < head) g[tid] = zero;
   if (tid < rest) g[tail + tid] = zero;
-  u32x4* out = reinterpret_cast<u32x4*>(g + head);
-  for (int64_t p = tid; p < pieces; p += kThreads) put16<kStream>(out + p, u32x4{0, 0, 0, 0});
+  for (int64_t p = tid; p < pieces; p += kThreads) put16<kStream>(g + head + p * kPiece<T>, u32x4{0, 0, 0, 0});
 }
 
 // One workgroup per row.
@@ -151,7 +150,6 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const T* logits, Rows
   }
   const T* x = logits + rows.at(row);
   const int64_t head = head_of(x, V), pieces = (V - head) / n, tail = head + pieces * n;
-  const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
   Running r{-FLT_MAX, 0.0};
   if (tid < head) {  // head < n <= 8 elements
     const float one[1] = {to_f32(x[tid])};
@@ -168,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const T* logits, Rows
 #pragma unroll
     for (int u = 0; u < kFlight; ++u) {
       const int64_t p = p0 + u * kThreads;
-      q[u].raw = body[p < pieces ? p : p0];
+      q[u].raw = get16(x + head + (p < pieces ? p : p0) * n);
     }
     if (p0 + (kFlight - 1) * kThreads < pieces) {
       float v[kFlight * n];
@@ -214,8 +212,7 @@ __device__ __forceinline__ void keep_packed(Piece<T> (&q)[P]) {
 
 // The policy loss with its gradient for a gradient of 1 of the loss, in one pass: a row stays in the
 // registers of its workgroup, P pieces a thread, between the maximum, the sum and the gradient, so
-// that logits are read once. inv_n is known before. Rows start and end on the same bytes of a 16-byte
-// piece in logits and grad.
+// that logits are read once. inv_n is known before.
 template <typename T, int kThreads, int P, bool kStream>
 __global__ __launch_bounds__(kThreads, P > 7 ? 4 : 8) void policy_grad_kernel(
     const T* logits, Rows rows, int64_t V, const int64_t* target, const uint8_t* mask, float k, Scale k2,
@@ -228,19 +225,17 @@ __global__ __launch_bounds__(kThreads, P > 7 ? 4 : 8) void policy_grad_kernel(
   T* g = grad + row * V;
   const int head = static_cast<int>(head_of(g, V)), pieces = static_cast<int>(V - head) / n;
   const int tail = head + pieces * n, rest = static_cast<int>(V) - tail;
-  u32x4* out = reinterpret_cast<u32x4*>(g + head);
   if (mask != nullptr && mask[row] == 0) {
     if (tid == 0) lp_out[row] = pol.term[row] = pol.coef[row] = 0.0f;
     write_zeros<T, kThreads, kStream>(g, head, tail, rest, pieces);
     return;
   }
   const T* x = logits + rows.at(row);
-  const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
   Piece<T> q[P];
 #pragma unroll
   for (int u = 0; u < P; ++u) {
     const int p = tid + u * kThreads;
-    q[u].raw = p < pieces ? body[p] : u32x4{0, 0, 0, 0};
+    q[u].raw = p < pieces ? get16(x + head + p * n) : u32x4{0, 0, 0, 0};
   }
   // the ends' elements, -inf where this thread has none: e^-inf adds nothing
   const float xh = tid < head ? to_f32(x[tid]) : -INFINITY;
@@ -321,7 +316,7 @@ __global__ __launch_bounds__(kThreads, P > 7 ? 4 : 8) void policy_grad_kernel(
           for (int i = 0; i < n; ++i)
             if (i == body_t % n) o.e[i] = from_f32<T>(hit(to_f32(q[u].e[i])));
         }
-        put16<kStream>(out + p, o.raw);
+        put16<kStream>(g + head + p * n, o.raw);
       }
     }
   };
@@ -475,7 +470,6 @@ __global__ __launch_bounds__(kThreads) void logprob_grad_kernel(
       if (scale1 != nullptr) c *= *scale1;
     }
     const int64_t head = head_of(g, V), pieces = (V - head) / n, tail = head + pieces * n;
-    u32x4* out = reinterpret_cast<u32x4*>(g + head);
     if (c == 0.0f) {
       write_zeros<T, kThreads, kStream>(g, head, tail, V - tail, pieces);
       continue;
@@ -488,19 +482,14 @@ __global__ __launch_bounds__(kThreads) void logprob_grad_kernel(
       const float e = k2.exp(v - st.x);
       return from_f32<T>(j == t ? fmaf(-cs, e, c) : -cs * e);
     };
-    if ((reinterpret_cast<uintptr_t>(x + head) & 15) != 0) {  // the rows' alignments differ
-      for (int64_t j = tid; j < V; j += kThreads) g[j] = one(j, to_f32(x[j]));
-      continue;
-    }
     if (tid < head) g[tid] = one(tid, to_f32(x[tid]));
     if (tid < V - tail) g[tail + tid] = one(tail + tid, to_f32(x[tail + tid]));
-    const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
     for (int64_t p0 = tid; p0 < pieces; p0 += 4 * kThreads) {
       Piece<T> q[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {  // 4 pieces in flight; past the row the first again
         const int64_t p = p0 + u * kThreads;
-        q[u].raw = body[p < pieces ? p : p0];
+        q[u].raw = get16(x + head + (p < pieces ? p : p0) * n);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -508,7 +497,7 @@ __global__ __launch_bounds__(kThreads) void logprob_grad_kernel(
         if (p >= pieces) break;
 #pragma unroll
         for (int i = 0; i < n; ++i) q[u].e[i] = one(head + p * n + i, to_f32(q[u].e[i]));
-        put16<kStream>(out + p, q[u].raw);
+        put16<kStream>(g + head + p * n, q[u].raw);
       }
     }
   }
@@ -568,15 +557,8 @@ int grad_launch(const void* logits, int32_t dtype, int64_t rows, int64_t inner, 
   return launch_status("logprob_grad_kernel");
 }
 
-// Whether policy_grad_kernel takes the rows: it holds them, and each row of logits starts at the same
-// place of a 16-byte piece as grad's.
-bool one_pass(const void* logits, const void* grad, int32_t dtype, int64_t rows, int64_t inner, int64_t V,
-              int64_t so, int64_t si) {
-  const int64_t size = dtype_size(dtype), n = 16 / size;
-  if (V > 16 * 1024 * n) return false;
-  if ((reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(grad)) % 16 != 0) return false;
-  return (inner == rows || (so - inner * V) % n == 0) && (si - V) % n == 0;
-}
+// Whether policy_grad_kernel holds a row.
+bool one_pass(int32_t dtype, int64_t V) { return V * dtype_size(dtype) <= 16 * 1024 * 16; }
 
 // Calls f with the threads of a row's workgroup and the pieces each holds, as compile-time constants.
 template <typename T, typename F>
@@ -633,7 +615,7 @@ extern "C" int lema_policy_loss(const void* logits, int32_t dtype, int64_t rows,
   LEMA_REQUIRE(aligned(grad, dtype_size(dtype)), "bad pointer");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Policy pol{old_lp, advantage, kl != 0.0f ? ref_lp : nullptr, term, coef, clip_low, clip_high, kl};
-  const bool fused = grad != nullptr && rows > 0 && one_pass(logits, grad, dtype, rows, inner, V, so, si);
+  const bool fused = grad != nullptr && rows > 0 && one_pass(dtype, V);
   policy_count_kernel<<<dim3(1), dim3(1024), 0, st>>>(mask, rows, scale, inv_n);
   if (fused) {
     for_dtype(dtype, [&](auto t) {

@@ -22,75 +22,43 @@ namespace {
 
 constexpr int64_t kMaxD = 16384;
 
-// Where lane `lane` of a row's W wavefronts finds its element k of step s: in 16-byte pieces, a load's
-// pieces next to each other (kVec), or single elements, a load's next to each other.
-template <typename T, int W, bool kVec>
+// Where lane `lane` of a row's W wavefronts finds its element k of step s: a load's units next to
+// each other.
+template <typename T, int W, int kKind>
 __device__ __forceinline__ int elem_at(int s, int k, int lane) {
-  constexpr int n = kVec ? kPiece<T> : 1;
+  constexpr int n = kUnit<T, kKind>;
   return ((s * 8 + k) / n * W * 64 + lane) * n + k % n;
 }
 
 // A row's elements as they come from memory, so that a row can be on its way while the one before
 // it is worked on.
-template <typename T, int W, int S, bool kVec>
-struct RawRow {
-  Piece<T> q[S * 8 / kPiece<T>];
-
+template <typename T, int W, int S, int kKind>
+struct RawRow : RowPart<T, kKind, S * 8> {
   template <bool kStream = false>
   __device__ __forceinline__ void fetch(const T* p, int D, int lane) {
-    constexpr int n = kPiece<T>;
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if constexpr (kVec) {
-#pragma unroll
-        for (int i = 0; i < 8 / n; ++i) {
-          const int e = elem_at<T, W, true>(s, i * n, lane);
-          q[s * 8 / n + i].raw = e < D ? get16<kStream>(p + e) : u32x4{0, 0, 0, 0};
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int e = elem_at<T, W, false>(s, k, lane);
-          q[(s * 8 + k) / n].e[k % n] = e < D ? p[e] : T{};
-        }
-      }
-    }
+    RowPart<T, kKind, S * 8>::template fetch<kStream>(p, D, [&](int i) { return elem_at<T, W, kKind>(0, i, lane); });
   }
-  __device__ __forceinline__ float at(int k) const { return to_f32(q[k / kPiece<T>].e[k % kPiece<T>]); }
+  __device__ __forceinline__ void settle(int D, int lane) {
+    RowPart<T, kKind, S * 8>::settle(D, [&](int i) { return elem_at<T, W, kKind>(0, i, lane); });
+  }
+  __device__ __forceinline__ float at(int k) const { return this->get(k); }
 };
 
-template <typename T, int W, int S, bool kVec>
+template <typename T, int W, int S, int kKind>
 __device__ __forceinline__ void load_row(const T* p, int D, int lane, float (&v)[S * 8]) {
-  RawRow<T, W, S, kVec> r;
+  RawRow<T, W, S, kKind> r;
   r.fetch(p, D, lane);
+  r.settle(D, lane);
 #pragma unroll
   for (int k = 0; k < S * 8; ++k) v[k] = r.at(k);
 }
 
-template <typename T, int W, int S, bool kVec, bool kStream = false>
+template <typename T, int W, int S, int kKind, bool kStream = false>
 __device__ __forceinline__ void store_row(T* p, int D, int lane, const float (&v)[S * 8]) {
+  RowPart<T, kKind, S * 8> r;
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    if constexpr (kVec) {
-      constexpr int n = kPiece<T>;
-#pragma unroll
-      for (int i = 0; i < 8 / n; ++i) {
-        const int e = elem_at<T, W, true>(s, i * n, lane);
-        if (e < D) {
-          Piece<T> q;
-#pragma unroll
-          for (int k = 0; k < n; ++k) q.e[k] = from_f32<T>(v[s * 8 + i * n + k]);
-          put16<kStream>(p + e, q.raw);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int e = elem_at<T, W, false>(s, k, lane);
-        if (e < D) p[e] = from_f32<T>(v[s * 8 + k]);
-      }
-    }
-  }
+  for (int k = 0; k < S * 8; ++k) r.set(k, v[k]);
+  r.template store<kStream>(p, D, [&](int i) { return elem_at<T, W, kKind>(0, i, lane); });
 }
 
 // Sums of N values over a row's W wavefronts, in every lane. `red` holds 2 * N * W floats, used
@@ -121,7 +89,7 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* red, int& turn) {
 // Wavefronts of a workgroup: a row each where a row takes one, else all on one row.
 constexpr int group_waves(int W) { return W > 1 ? W : 4; }
 
-template <typename T, int W, int S, bool kVec>
+template <typename T, int W, int S, int kKind>
 __global__ __launch_bounds__(64 * group_waves(W)) void layer_norm_kernel(
     const T* x, const T* d, const T* w, const T* b, float eps, int64_t rows, int D, T* s_out, T* h_out) {
   __shared__ float red[2 * W];
@@ -131,12 +99,12 @@ __global__ __launch_bounds__(64 * group_waves(W)) void layer_norm_kernel(
   if (row >= rows) return;
   int turn = 0;
   float v[S * 8], t[S * 8];
-  load_row<T, W, S, kVec>(x + row * D, D, lane, v);
+  load_row<T, W, S, kKind>(x + row * D, D, lane, v);
   if (d != nullptr) {
-    load_row<T, W, S, kVec>(d + row * D, D, lane, t);
+    load_row<T, W, S, kKind>(d + row * D, D, lane, t);
 #pragma unroll
     for (int k = 0; k < S * 8; ++k) v[k] = to_f32(from_f32<T>(v[k] + t[k]));
-    store_row<T, W, S, kVec>(s_out + row * D, D, lane, v);
+    store_row<T, W, S, kKind>(s_out + row * D, D, lane, v);
   }
   float sum[1] = {0.0f};
 #pragma unroll
@@ -149,24 +117,24 @@ __global__ __launch_bounds__(64 * group_waves(W)) void layer_norm_kernel(
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       v[s * 8 + k] -= m;
-      if (elem_at<T, W, kVec>(s, k, lane) < D) sum[0] += v[s * 8 + k] * v[s * 8 + k];
+      if (elem_at<T, W, kKind>(s, k, lane) < D) sum[0] += v[s * 8 + k] * v[s * 8 + k];
     }
   row_sums<W, 1>(sum, red, turn);
   const float r = rsqrtf(sum[0] / static_cast<float>(D) + eps);
-  if (w != nullptr) load_row<T, W, S, kVec>(w, D, lane, t);
+  if (w != nullptr) load_row<T, W, S, kKind>(w, D, lane, t);
 #pragma unroll
   for (int k = 0; k < S * 8; ++k) v[k] *= w != nullptr ? r * t[k] : r;
   if (b != nullptr) {
-    load_row<T, W, S, kVec>(b, D, lane, t);
+    load_row<T, W, S, kKind>(b, D, lane, t);
 #pragma unroll
     for (int k = 0; k < S * 8; ++k) v[k] += t[k];
   }
-  store_row<T, W, S, kVec>(h_out + row * D, D, lane, v);
+  store_row<T, W, S, kKind>(h_out + row * D, D, lane, v);
 }
 
 // Rows blockIdx.x * kSlots + slot, then on by gridDim.x * kSlots. partial: [2, gridDim.x, D] fp32,
 // this workgroup's sums of gh z and of gh, where wanted.
-template <typename T, int W, int S, bool kVec, bool kCenter, bool kStream>
+template <typename T, int W, int S, int kKind, bool kCenter, bool kStream>
 __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
     const T* s_in, const T* w, const T* gh, const T* gs, float eps, int64_t rows, int D, T* gx,
     float* partial) {
@@ -180,10 +148,10 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
   float wv[S * 8], gw[S * 8], gb[S * 8];
 #pragma unroll
   for (int k = 0; k < S * 8; ++k) gw[k] = gb[k] = 0.0f, wv[k] = 1.0f;
-  if (w != nullptr) load_row<T, W, S, kVec>(w, D, lane, wv);
+  if (w != nullptr) load_row<T, W, S, kKind>(w, D, lane, wv);
   const int64_t step = static_cast<int64_t>(gridDim.x) * kSlots;
   int64_t row = static_cast<int64_t>(blockIdx.x) * kSlots + slot;
-  RawRow<T, W, S, kVec> next_v, next_g, next_gs;
+  RawRow<T, W, S, kKind> next_v, next_g, next_gs;
   const bool add = gx != nullptr && gs != nullptr;
   const auto fetch = [&](int64_t r) {
     next_v.template fetch<kStream>(s_in + r * D, D, lane);
@@ -195,7 +163,9 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
   for (; row < rows; row += step) {
     if (!kAhead) fetch(row);
     float v[S * 8], g[S * 8];
-    const RawRow<T, W, S, kVec> gs_row = next_gs;
+    RawRow<T, W, S, kKind> gs_row = next_gs;
+    next_v.settle(D, lane);
+    next_g.settle(D, lane);
 #pragma unroll
     for (int k = 0; k < S * 8; ++k) {
       v[k] = next_v.at(k);
@@ -212,7 +182,7 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
       for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          v[s * 8 + k] = elem_at<T, W, kVec>(s, k, lane) < D ? v[s * 8 + k] - m : 0.0f;
+          v[s * 8 + k] = elem_at<T, W, kKind>(s, k, lane) < D ? v[s * 8 + k] - m : 0.0f;
     }
     float sum[3] = {0.0f, 0.0f, 0.0f};  // of squares, of a v, of a
 #pragma unroll
@@ -234,10 +204,11 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
     }
     if (gx != nullptr) {
       if (add) {
+        gs_row.settle(D, lane);
 #pragma unroll
         for (int k = 0; k < S * 8; ++k) v[k] += gs_row.at(k);
       }
-      store_row<T, W, S, kVec, kStream>(gx + row * D, D, lane, v);
+      store_row<T, W, S, kKind, kStream>(gx + row * D, D, lane, v);
     }
   }
   if (partial == nullptr) return;
@@ -249,7 +220,7 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
       for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int e = elem_at<T, W, kVec>(s, k, lane);
+          const int e = elem_at<T, W, kKind>(s, k, lane);
           comb[slot * 512 * S + e] = which ? gb[s * 8 + k] : gw[s * 8 + k];
         }
       __syncthreads();
@@ -264,7 +235,7 @@ __global__ __launch_bounds__(64 * group_waves(W)) void norm_grad_kernel(
       for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int e = elem_at<T, W, kVec>(s, k, lane);
+          const int e = elem_at<T, W, kKind>(s, k, lane);
           if (e < D) out[e] = which ? gb[s * 8 + k] : gw[s * 8 + k];
         }
     }
@@ -353,10 +324,15 @@ int64_t grad_groups(int64_t rows, int64_t D) {
   return want < fit ? want : fit;
 }
 
-bool pieces_ok(int64_t D, std::initializer_list<const void*> ptrs) {
-  bool ok = D % 8 == 0;
-  for (const void* p : ptrs) ok = ok && aligned(p, 16);  // NULL counts as aligned
-  return ok;
+// Up to four tensors of rows pass through. Where they are far larger than the Infinity Cache they go
+// past it: the gradient of 65,536 rows of 1536 in bf16 took 137 us, not 159, and the norm that ran next
+// 133, not 130. 8192 rows of 4096 in fp16 fit it and lost by it, 59 us against 56 (and 49 against 44).
+// So do rows that start inside a piece, whose lines are then fetched by each of the wavefronts that share
+// them: 65,536 of 1535 took 542 us.
+bool past_cache(int64_t rows, int64_t D, int64_t size, std::initializer_list<const void*> tensors) {
+  bool whole = D % 8 == 0;
+  for (const void* p : tensors) whole = whole && aligned(p, 16);  // NULL counts as aligned
+  return whole && rows * D * size > (int64_t(128) << 20);
 }
 
 int check_rows(int32_t dtype, int64_t rows, int64_t D) {
@@ -382,17 +358,19 @@ extern "C" int lema_layer_norm(const void* x, const void* d, const void* w, cons
   const int size = dtype_size(dtype);
   for (const void* p : {x, d, w, b, static_cast<const void*>(s_out), static_cast<const void*>(h_out)})
     LEMA_REQUIRE(aligned(p, size), "pointers must be aligned to an element");
-  const bool vec = pieces_ok(D, {x, d, w, b, s_out, h_out});
+  const RowKind kind = row_kind(dtype, D);
   for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     for_width(D, [&](auto wc, auto sc) {
       constexpr int W = decltype(wc)::value, S = decltype(sc)::value;
       const int64_t slots = group_waves(W) / W, grid = (rows + slots - 1) / slots;
-      const auto kernel = vec ? layer_norm_kernel<T, W, S, true> : layer_norm_kernel<T, W, S, false>;
-      kernel<<<dim3(grid), dim3(64 * group_waves(W)), 0, static_cast<hipStream_t>(stream)>>>(
-          static_cast<const T*>(x), static_cast<const T*>(d), static_cast<const T*>(w),
-          static_cast<const T*>(b), eps, rows, static_cast<int>(D), static_cast<T*>(s_out),
-          static_cast<T*>(h_out));
+      for_kind<T>(kind, [&](auto k) {
+        layer_norm_kernel<T, W, S, decltype(k)::value>
+            <<<dim3(grid), dim3(64 * group_waves(W)), 0, static_cast<hipStream_t>(stream)>>>(
+                static_cast<const T*>(x), static_cast<const T*>(d), static_cast<const T*>(w),
+                static_cast<const T*>(b), eps, rows, static_cast<int>(D), static_cast<T*>(s_out),
+                static_cast<T*>(h_out));
+      });
     });
   });
   return launch_status("layer_norm_kernel");
@@ -425,26 +403,26 @@ extern "C" int lema_norm_grad(const void* s, const void* w, const void* gh, cons
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t groups = rows > 0 ? grad_groups(rows, D) : 0;
   float* partial = sums ? static_cast<float*>(workspace) : nullptr;
-  const bool vec = pieces_ok(D, {s, w, gh, gs, gx});
-  // Up to four tensors of rows pass through. Where they are far larger than the Infinity Cache they
-  // go past it: 65,536 rows of 1536 in bf16 took 137 us, not 159, and the norm that ran next 133, not
-  // 130. 8192 rows of 4096 in fp16 fit it and lost by it, 59 us against 56 (and 49 against 44).
-  const bool stream_rows = rows * D * size > (int64_t(128) << 20);
+  const RowKind kind = row_kind(dtype, D);
+  const bool stream_rows = past_cache(rows, D, size, {s, gh, gs, gx});
   for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     if (rows > 0)
       for_grad_width(D, [&](auto wc, auto sc) {
         constexpr int W = decltype(wc)::value, S = decltype(sc)::value;
-        const auto kernel =
-            center ? (!vec     ? norm_grad_kernel<T, W, S, false, true, false>
-                      : stream_rows ? norm_grad_kernel<T, W, S, true, true, true>
-                                    : norm_grad_kernel<T, W, S, true, true, false>)
-                   : (!vec     ? norm_grad_kernel<T, W, S, false, false, false>
-                      : stream_rows ? norm_grad_kernel<T, W, S, true, false, true>
-                                    : norm_grad_kernel<T, W, S, true, false, false>);
-        kernel<<<dim3(groups), dim3(64 * group_waves(W)), 0, st>>>(
-            static_cast<const T*>(s), static_cast<const T*>(w), static_cast<const T*>(gh),
-            static_cast<const T*>(gs), eps, rows, static_cast<int>(D), static_cast<T*>(gx), partial);
+        const auto launch = [&](auto kernel) {
+          kernel<<<dim3(groups), dim3(64 * group_waves(W)), 0, st>>>(
+              static_cast<const T*>(s), static_cast<const T*>(w), static_cast<const T*>(gh),
+              static_cast<const T*>(gs), eps, rows, static_cast<int>(D), static_cast<T*>(gx), partial);
+        };
+        if (stream_rows)
+          launch(center ? norm_grad_kernel<T, W, S, kWholeRows, true, true>
+                        : norm_grad_kernel<T, W, S, kWholeRows, false, true>);
+        else
+          for_kind<T>(kind, [&](auto k) {
+            launch(center ? norm_grad_kernel<T, W, S, decltype(k)::value, true, false>
+                          : norm_grad_kernel<T, W, S, decltype(k)::value, false, false>);
+          });
       });
     if (sums)
       norm_weight_kernel<T><<<dim3((D + 15) / 16, gb != nullptr ? 2 : 1), dim3(1024), 0, st>>>(
