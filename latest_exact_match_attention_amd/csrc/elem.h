@@ -75,7 +75,7 @@ __device__ __forceinline__ void put16(T* p, u32x4 v) {
 //   kRaggedRows  16-bit types, D >= 8: pieces too. What would reach past the row is read as the row's
 //                last whole piece instead and shifted into place once it is used, so that no load is
 //                conditional: a branch around the last one made the kernels wait for every load where
-//                it was issued (the gradient of 65,536 norms of 1535 in bf16: 489 us, 217 so).
+//                it was issued (the gradient of 65,536 norms of 1535 in bf16: 489 us, 218 so).
 //   kElements    element by element: fp32 rows, where 64 lanes' elements are whole lines anyway
 //                and pieces that straddle lines cost more (18 us for the gradient of 4099 layer norms of
 //                1001, 14 so), and rows shorter than a piece.

@@ -324,17 +324,6 @@ int64_t grad_groups(int64_t rows, int64_t D) {
   return want < fit ? want : fit;
 }
 
-// Up to four tensors of rows pass through. Where they are far larger than the Infinity Cache they go
-// past it: the gradient of 65,536 rows of 1536 in bf16 took 137 us, not 159, and the norm that ran next
-// 133, not 130. 8192 rows of 4096 in fp16 fit it and lost by it, 59 us against 56 (and 49 against 44).
-// So do rows that start inside a piece, whose lines are then fetched by each of the wavefronts that share
-// them: 65,536 of 1535 took 542 us.
-bool past_cache(int64_t rows, int64_t D, int64_t size, std::initializer_list<const void*> tensors) {
-  bool whole = D % 8 == 0;
-  for (const void* p : tensors) whole = whole && aligned(p, 16);  // NULL counts as aligned
-  return whole && rows * D * size > (int64_t(128) << 20);
-}
-
 int check_rows(int32_t dtype, int64_t rows, int64_t D) {
   LEMA_REQUIRE(dtype_size(dtype) != 0, "unknown dtype %d", dtype);
   LEMA_REQUIRE(D > 0 && D <= kMaxD, "row length %lld must lie in [1, %lld]", (long long)D,
@@ -404,7 +393,11 @@ extern "C" int lema_norm_grad(const void* s, const void* w, const void* gh, cons
   const int64_t groups = rows > 0 ? grad_groups(rows, D) : 0;
   float* partial = sums ? static_cast<float*>(workspace) : nullptr;
   const RowKind kind = row_kind(dtype, D);
-  const bool stream_rows = past_cache(rows, D, size, {s, gh, gs, gx});
+  // Up to four tensors of rows pass through. Where they are far larger than the Infinity Cache they go
+  // past it: the gradient of 65,536 rows of 1536 in bf16 took 137 us, not 159 (of 1535: 200, not 218),
+  // and the norm that ran next 133, not 130. 8192 rows of 4096 in fp16 fit it and lost by it, 59 us
+  // against 56 (and 49 against 44).
+  const bool past = rows * D * size > (int64_t(128) << 20);
   for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     if (rows > 0)
@@ -415,14 +408,16 @@ extern "C" int lema_norm_grad(const void* s, const void* w, const void* gh, cons
               static_cast<const T*>(s), static_cast<const T*>(w), static_cast<const T*>(gh),
               static_cast<const T*>(gs), eps, rows, static_cast<int>(D), static_cast<T*>(gx), partial);
         };
-        if (stream_rows)
-          launch(center ? norm_grad_kernel<T, W, S, kWholeRows, true, true>
-                        : norm_grad_kernel<T, W, S, kWholeRows, false, true>);
-        else
-          for_kind<T>(kind, [&](auto k) {
-            launch(center ? norm_grad_kernel<T, W, S, decltype(k)::value, true, false>
-                          : norm_grad_kernel<T, W, S, decltype(k)::value, false, false>);
-          });
+        for_kind<T>(kind, [&](auto k) {
+          constexpr int kKind = decltype(k)::value;
+          constexpr bool kCan = kKind != kElements;
+          if (kCan && past)
+            launch(center ? norm_grad_kernel<T, W, S, kKind, true, kCan>
+                          : norm_grad_kernel<T, W, S, kKind, false, kCan>);
+          else
+            launch(center ? norm_grad_kernel<T, W, S, kKind, true, false>
+                          : norm_grad_kernel<T, W, S, kKind, false, false>);
+        });
       });
     if (sums)
       norm_weight_kernel<T><<<dim3((D + 15) / 16, gb != nullptr ? 2 : 1), dim3(1024), 0, st>>>(
