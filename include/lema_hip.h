@@ -256,7 +256,8 @@ int lema_embedding(const void* table, int32_t dtype, int64_t vocab, int64_t D, c
 /* The table's gradient: gw row v = scale * sum of gy row i over the positions i with ids[i] = v,
  * summed in fp32 in a fixed order and rounded once; every row is written, zeros for tokens that
  * do not occur and for token `padding` (negative: none). Ids outside [0, vocab) take no part.
- *   gy   contiguous [n, D] of `dtype`; n < 2^31 - 16384, vocab and D at most 2^20
+ *   gy   contiguous [n, D] of `dtype`; n < 2^31 - 16384, vocab and D at most 2^20,
+ *        (n / 16 + vocab) * ceil(D / 1536) < 2^26
  *   workspace  256-byte aligned, lema_embedding_grad_workspace_bytes(n, vocab, D) bytes: about
  *              16 bytes a position, 4 a token, and n / 64 rows of fp32 (n / 16 up to 16384
  *              positions), padded to 512 */

@@ -30,6 +30,16 @@ __device__ __forceinline__ Bf16 from_f32<Bf16>(float f) {
   return Bf16{__builtin_bit_cast(uint16_t, static_cast<__bf16>(f))};
 }
 
+// A grid of n workgroups or more, and a workgroup's index in it: a dimension takes fewer than 2^32
+// threads, which rows of a few elements reach within the memory there is.
+inline dim3 blocks_of(int64_t n) {
+  const int64_t x = n < (1 << 21) ? n : 1 << 21;
+  return dim3(static_cast<uint32_t>(x), static_cast<uint32_t>((n + x - 1) / x));
+}
+__device__ __forceinline__ int64_t block_index() {
+  return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+}
+
 template <typename T>
 constexpr int kPiece = 16 / static_cast<int>(sizeof(T));  // elements of a 16-byte piece
 

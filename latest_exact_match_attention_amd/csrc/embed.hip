@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void embed_kernel(const T* table, int64_t voca
                                                     const int64_t* ids, int64_t n, int slices,
                                                     float scale, T* out) {
   const int lane = threadIdx.x & 63;
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + wave_index();
+  const int64_t u = block_index() * 4 + wave_index();
   const int64_t i = u / slices;
   if (i >= n) return;
   const int64_t c0 = (u - i * slices) * kCols, id = ids[i];
@@ -517,7 +517,7 @@ int embed_launch(const void* table, int32_t dtype, int64_t vocab, int64_t D, con
   for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const auto launch = [&](auto kernel) {
-      kernel<<<dim3(grid), dim3(256), 0, st>>>(static_cast<const T*>(table), vocab, D, ids, n,
+      kernel<<<blocks_of(grid), dim3(256), 0, st>>>(static_cast<const T*>(table), vocab, D, ids, n,
                                                static_cast<int>(slices), scale, static_cast<T*>(out));
     };
     for_kind<T>(kind, [&](auto k) {
@@ -581,7 +581,7 @@ extern "C" int lema_embedding_grad(const void* gy, int32_t dtype, const int64_t*
   // a wavefront takes up to 3 slices: its chain of reads (start, positions, rows) is then shared
   const int64_t per = cols < 3 ? cols : 3, slices = (cols + per - 1) / per;
   const int64_t grid = ((tiles + vocab) * slices + 3) / 4;
-  LEMA_REQUIRE(grid < (int64_t(1) << 31), "table [%lld, %lld] is too large", (long long)vocab,
+  LEMA_REQUIRE(grid < (int64_t(1) << 24), "table [%lld, %lld] is too large", (long long)vocab,
                (long long)D);
   if (o.spans > 1) embed_count_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
   embed_scatter_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);

@@ -132,13 +132,15 @@ __device__ __forceinline__ void write_zeros(T* g, int64_t head, int64_t tail, in
 
 // One workgroup per row.
 template <typename T, int kThreads>
-__global__ __launch_bounds__(kThreads) void logprob_kernel(const T* logits, Rows rows, int64_t V,
-                                                           const int64_t* target, const uint8_t* mask,
+__global__ __launch_bounds__(kThreads) void logprob_kernel(const T* logits, Rows rows, int64_t count,
+                                                           int64_t V, const int64_t* target,
+                                                           const uint8_t* mask,
                                                            float temperature, Scale k2, float* lp_out,
                                                            double* lp64_out, float2* stats, Policy pol) {
   constexpr int kWaves = kThreads / 64, n = kPiece<T>;
   __shared__ Running part[kWaves];
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_index();
+  if (row >= count) return;
   const int tid = threadIdx.x;
   if (mask != nullptr && mask[row] == 0) {
     if (tid == 0) {
@@ -215,12 +217,13 @@ __device__ __forceinline__ void keep_packed(Piece<T> (&q)[P]) {
 // that logits are read once. inv_n is known before.
 template <typename T, int kThreads, int P, bool kStream>
 __global__ __launch_bounds__(kThreads, P > 7 ? 4 : 8) void policy_grad_kernel(
-    const T* logits, Rows rows, int64_t V, const int64_t* target, const uint8_t* mask, float k, Scale k2,
-    float* lp_out, float2* stats, Policy pol, const float* inv_n, T* grad) {
+    const T* logits, Rows rows, int64_t count, int64_t V, const int64_t* target, const uint8_t* mask,
+    float k, Scale k2, float* lp_out, float2* stats, Policy pol, const float* inv_n, T* grad) {
   constexpr int kWaves = kThreads / 64, n = kPiece<T>;
   __shared__ float part[2][kWaves];
   __shared__ float coef;
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_index();
+  if (row >= count) return;
   const int tid = threadIdx.x;
   T* g = grad + row * V;
   const int head = static_cast<int>(head_of(g, V)), pieces = static_cast<int>(V - head) / n;
@@ -530,8 +533,8 @@ int logprob_launch(const void* logits, int32_t dtype, int64_t rows, int64_t inne
     using T = decltype(t);
     const bool wide = wide_rows(dtype, V);
     const auto kernel = wide ? logprob_kernel<T, 1024> : logprob_kernel<T, 256>;
-    kernel<<<dim3(rows), dim3(wide ? 1024 : 256), 0, st>>>(
-        static_cast<const T*>(logits), Rows{inner, so, si}, V, target, mask, temperature,
+    kernel<<<blocks_of(rows), dim3(wide ? 1024 : 256), 0, st>>>(
+        static_cast<const T*>(logits), Rows{inner, so, si}, rows, V, target, mask, temperature,
         Scale(temperature), lp, lp64, reinterpret_cast<float2*>(stats), pol);
   });
   return launch_status("logprob_kernel");
@@ -548,7 +551,7 @@ int grad_launch(const void* logits, int32_t dtype, int64_t rows, int64_t inner, 
     const auto kernel = wide ? (past ? logprob_grad_kernel<T, 1024, true> : logprob_grad_kernel<T, 1024, false>)
                              : (past ? logprob_grad_kernel<T, 256, true> : logprob_grad_kernel<T, 256, false>);
     // where nothing is likely to be left to do, few workgroups (16,384 that end at once take 17 us)
-    const int64_t grid = unit_done && rows > 512 ? 512 : rows;
+    const int64_t most = unit_done ? 512 : 1 << 21, grid = rows < most ? rows : most;
     kernel<<<dim3(grid), dim3(wide ? 1024 : 256), 0, st>>>(
         static_cast<const T*>(logits), Rows{inner, so, si}, rows, V, target, mask, 1.0f / temperature,
         Scale(temperature), reinterpret_cast<const float2*>(stats), coef, per, scale0, scale1, unit_done,
@@ -625,8 +628,8 @@ extern "C" int lema_policy_loss(const void* logits, int32_t dtype, int64_t rows,
         const auto kernel = rows * V * static_cast<int64_t>(sizeof(T)) > kStreamBytes
                                 ? policy_grad_kernel<T, kThreads, P, true>
                                 : policy_grad_kernel<T, kThreads, P, false>;
-        kernel<<<dim3(rows), dim3(kThreads), 0, st>>>(
-            static_cast<const T*>(logits), Rows{inner, so, si}, V, target, mask, 1.0f / temperature,
+        kernel<<<blocks_of(rows), dim3(kThreads), 0, st>>>(
+            static_cast<const T*>(logits), Rows{inner, so, si}, rows, V, target, mask, 1.0f / temperature,
             Scale(temperature), lp, reinterpret_cast<float2*>(stats), pol, inv_n,
             static_cast<T*>(grad));
       });

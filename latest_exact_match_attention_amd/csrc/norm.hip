@@ -95,7 +95,7 @@ __global__ __launch_bounds__(64 * group_waves(W)) void layer_norm_kernel(
   __shared__ float red[2 * W];
   constexpr int kSlots = group_waves(W) / W;
   const int lane = W > 1 ? threadIdx.x : threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kSlots + (W > 1 ? 0 : threadIdx.x >> 6);
+  const int64_t row = block_index() * kSlots + (W > 1 ? 0 : threadIdx.x >> 6);
   if (row >= rows) return;
   int turn = 0;
   float v[S * 8], t[S * 8];
@@ -355,7 +355,7 @@ extern "C" int lema_layer_norm(const void* x, const void* d, const void* w, cons
       const int64_t slots = group_waves(W) / W, grid = (rows + slots - 1) / slots;
       for_kind<T>(kind, [&](auto k) {
         layer_norm_kernel<T, W, S, decltype(k)::value>
-            <<<dim3(grid), dim3(64 * group_waves(W)), 0, static_cast<hipStream_t>(stream)>>>(
+            <<<blocks_of(grid), dim3(64 * group_waves(W)), 0, static_cast<hipStream_t>(stream)>>>(
                 static_cast<const T*>(x), static_cast<const T*>(d), static_cast<const T*>(w),
                 static_cast<const T*>(b), eps, rows, static_cast<int>(D), static_cast<T*>(s_out),
                 static_cast<T*>(h_out));

@@ -105,6 +105,13 @@ def test_gradient_of_the_largest(dev, dtype, n, V, D):
     check_grad(gw, ids, gy, V, 1.0)
 
 
+def test_more_positions_than_one_grid_dimension(dev):
+    emb, g = table(dev, 300, 8, torch.bfloat16, seed=5)
+    ids = torch.randint(0, 300, ((1 << 23) + 5,), device=dev, generator=g)
+    with torch.no_grad():
+        assert torch.equal(embed(emb, ids), emb.weight[ids])
+
+
 @pytest.mark.parametrize("n", [31, 32, 33, 63, 64, 65, 97, 127, 128, 200, 5000, 40000])
 def test_gradient_one_token(dev, n):
     """Every position the same token: lists around the longest that one wavefront adds up."""

@@ -69,6 +69,28 @@ def test_token_logprobs(dev, dtype, V, temperature):
     check_grad(grad, p, targets, c.double(), 0 * lp, temperature, sum_err)
 
 
+def test_more_rows_than_one_grid_dimension(dev):
+    """Short rows, 2.1 million of them: every one as in a call of a few. A loss scaled by their
+    repetitions has the same factor, 1 / 1031 rounded once, and so the same gradient."""
+    n = 2035
+    logits, targets, g = make(dev, (1031,), 8, torch.float16, seed=3)
+    many, many_t = logits.repeat(n, 1).requires_grad_(True), targets.repeat(n)
+    logits.requires_grad_(True)
+    c, z = torch.randn(1031, device=dev, generator=g), torch.zeros(1031, device=dev)
+    small = token_logprobs(logits, targets)
+    got = token_logprobs(many, many_t)
+    assert torch.equal(got.view(n, 1031), small.expand(n, -1))
+    (want,) = torch.autograd.grad(small, [logits], c)
+    (grad,) = torch.autograd.grad(got, [many], c.repeat(n))
+    assert torch.equal(grad.view(n, 1031, 8), want.expand(n, -1, -1))
+    small = policy_loss(logits, targets, z, c)
+    got = policy_loss(many, many_t, z.repeat(n), c.repeat(n), scale=float(n))
+    assert torch.equal(got.logprobs.view(n, 1031), small.logprobs.expand(n, -1))
+    (want,) = torch.autograd.grad(small.loss, [logits])
+    (grad,) = torch.autograd.grad(got.loss, [many])
+    assert torch.equal(grad.view(n, 1031, 8), want.expand(n, -1, -1))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_layouts(dev, dtype):
     """Slices along any dim, odd row starts, expanded rows, a transposed vocabulary."""

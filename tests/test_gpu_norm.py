@@ -96,6 +96,20 @@ def test_row_counts(dev, rows, D):
     check(norm, True, s.detach(), gh, gs, h.detach(), gx, gw, gb)
 
 
+def test_more_rows_than_one_grid_dimension(dev):
+    """Short rows, 8.4 million of them: every one as in a call of a few."""
+    norm, x, _, gh, _ = make(dev, (4099, 8), torch.bfloat16, True, seed=8)
+    n = 2047
+    small, _ = layer_norm(x, norm)
+    xs = x.repeat(n, 1).requires_grad_(True)
+    h, _ = layer_norm(xs, norm)
+    assert torch.equal(h.detach().view(n, 4099, 8), small.detach().expand(n, -1, -1))
+    x.requires_grad_(True)
+    (want,) = torch.autograd.grad(layer_norm(x, norm)[0], [x], gh)
+    (gx,) = torch.autograd.grad(h, [xs], gh.repeat(n, 1))
+    assert torch.equal(gx.view(n, 4099, 8), want.expand(n, -1, -1))
+
+
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("rows,D", [(1, 8), (3, 512), (70, 520), (5000, 1536), (33, 2048), (9, 2056),
                                     (600, 4096)])
