@@ -783,7 +783,8 @@ def lm_loss(model: Transformer, x: torch.Tensor, y: torch.Tensor, chunk: int = 4
     head and the loss run `chunk` positions at a time on the final hidden states, in fp32
     (code/lema/train.py:131-152). Differentiable; a backward keeps the chunks' logits until then.
     At B4 T16384 with a 50,304-word vocabulary, chunks of 4096 positions (head GEMMs of 16,384
-    rows, 1.65 GB of bf16 logits at a time) took the whole forward from 119.9-120.4 to 118.2-118.8 ms against chunks of 1024."""
+    rows, 1.65 GB of bf16 logits at a time) took the whole forward from 119.9-120.4 to
+    118.2-118.8 ms against chunks of 1024."""
     h = model.hidden(x)
     total = torch.zeros((), dtype=torch.float32, device=h.device)
     for a in range(0, x.shape[1], chunk):

@@ -105,6 +105,22 @@ def test_gradient_of_the_largest(dev, dtype, n, V, D):
     check_grad(gw, ids, gy, V, 1.0)
 
 
+@pytest.mark.parametrize("half", [520, 515])
+def test_rows_past_the_cache(dev, half):
+    """Rows and a table of more than 256 MB: the columns as in calls of half of them."""
+    n, V, D = 100001, 32003, 2 * half
+    emb, g = table(dev, V, D, torch.bfloat16, seed=half)
+    ids = (torch.rand(n, device=dev, generator=g) ** 3 * V).long()
+    gy = torch.randn(n, D, device=dev, generator=g).to(torch.bfloat16)
+    y = embed(emb, ids)
+    assert torch.equal(y, emb.weight[ids])
+    (gw,) = torch.autograd.grad(y, [emb.weight], gy)
+    for cols in (slice(0, half), slice(half, D)):
+        part = torch.nn.Embedding(V, half, _weight=emb.weight.detach()[:, cols].contiguous())
+        (want,) = torch.autograd.grad(embed(part, ids), [part.weight], gy[:, cols])
+        assert torch.equal(gw[:, cols], want)
+
+
 def test_more_positions_than_one_grid_dimension(dev):
     emb, g = table(dev, 300, 8, torch.bfloat16, seed=5)
     ids = torch.randint(0, 300, ((1 << 23) + 5,), device=dev, generator=g)

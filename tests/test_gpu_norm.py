@@ -96,6 +96,24 @@ def test_row_counts(dev, rows, D):
     check(norm, True, s.detach(), gh, gs, h.detach(), gx, gw, gb)
 
 
+@pytest.mark.parametrize("D", [1530, 1528])
+@pytest.mark.parametrize("start", [0, 1])
+def test_rows_past_the_cache(dev, D, start):
+    """Tensors of more than 128 MB, from any element on: every row as in calls of a few."""
+    rows = 44001
+    norm, x, _, gh, _ = make(dev, (rows * D + 8,), torch.bfloat16, True, seed=D)
+    norm, *_ = make(dev, (1, D), torch.bfloat16, True, seed=D)
+    x, gh = (t[start:start + rows * D].view(rows, D) for t in (x, gh))
+    leaf = x.detach().requires_grad_(True)
+    h, _ = layer_norm(leaf, norm)
+    (gx,) = torch.autograd.grad(h, [leaf], gh)
+    for i in range(0, rows, 11000):
+        part = x[i:i + 11000].detach().requires_grad_(True)
+        want, _ = layer_norm(part, norm)
+        assert torch.equal(h[i:i + 11000], want)
+        assert torch.equal(gx[i:i + 11000], torch.autograd.grad(want, [part], gh[i:i + 11000])[0])
+
+
 def test_more_rows_than_one_grid_dimension(dev):
     """Short rows, 8.4 million of them: every one as in a call of a few."""
     norm, x, _, gh, _ = make(dev, (4099, 8), torch.bfloat16, True, seed=8)
