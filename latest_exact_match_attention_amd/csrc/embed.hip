@@ -8,14 +8,15 @@
 //   count    per span of positions, how many fall into each of up to 1024 buckets of tokens
 //            (the token's high bits);
 //   scatter  each span puts its positions, in order, into the buckets;
-//   order    each bucket orders its positions by token, and notes where each token's start;
+//   order    each bucket orders its positions by token, and notes where each token's start. Of up to
+//            7168 positions each bucket picks its own, and there is no count and no scatter;
 //   sum      a wavefront per (token, 512 columns) adds up to 32 rows. A longer list would
 //            keep one wavefront busy while the others end, so its whole tiles of 16 or 64 positions are
 //            summed by wavefronts of their own, in the same launch, in fp32;
 //   join     a workgroup per (long list, 512 columns) adds its tiles and its ragged ends.
 // A wavefront keeps its own cursors, so a place is a ballot per bit of the digit and needs no
 // atomics. gy is read once and the table's gradient written once, which bounds the work (HBM);
-// the ordering costs three short launches.
+// the ordering costs one or three short launches.
 #include "elem.h"
 
 namespace lema {
@@ -25,6 +26,10 @@ constexpr int kBuckets = 1024;      // at most, of 1 << row_bits tokens each
 constexpr int kMaxRowBits = 10;     // so at most 2^20 tokens
 constexpr int kSpanStep = 1024;     // a span is a multiple of it: 16 wavefronts of 64
 constexpr int kLong = 32;           // positions of a token that one wavefront adds up
+// Up to this many positions every bucket reads all of them, 15 a lane at once: 5003 of a table of 32,003
+// took 12 us so and 16 in three launches, whose host side is 5 us longer (a pass with its gradient 87
+// and 95 us). At most what leaves a bucket's items and cursors within 64 KB.
+constexpr int64_t kShort = 7168;
 constexpr int kCols = 512;          // columns of a wavefront, 8 a lane
 
 __device__ __forceinline__ int wave_index() {
@@ -93,6 +98,7 @@ struct Order {            // what the ordering kernels share
   uint32_t* perm;         // [n] positions by (token, position)
   uint32_t* token;        // [n] their tokens
   uint32_t* start;        // [vocab + 1]
+  bool pick;              // n is up to kShort: what follows is not filled
   uint32_t* long_count;   // lists of more than kLong
   uint32_t* long_list;    // their tokens, starts and ends, in no order
 };
@@ -195,20 +201,15 @@ __global__ __launch_bounds__(1024) void embed_scatter_kernel(Order o) {
   });
   // thread t: bucket t's positions in all spans, and in the spans before this one
   uint32_t all = 0, before = 0;
-  if (o.spans == 1) {  // not counted before: the sixteenths just counted are all there is
-    __syncthreads();
-    for (int k = 0; k < 16; ++k) all += cur[k][t];
-  } else {
-    for (int s0 = 0; s0 < o.spans; s0 += 32) {
-      uint32_t c[32];
+  for (int s0 = 0; s0 < o.spans; s0 += 32) {
+    uint32_t c[32];
 #pragma unroll
-      for (int u = 0; u < 32; ++u)
-        c[u] = o.counts[static_cast<int64_t>(s0 + u < o.spans ? s0 + u : s0) * kBuckets + t];
+    for (int u = 0; u < 32; ++u)
+      c[u] = o.counts[static_cast<int64_t>(s0 + u < o.spans ? s0 + u : s0) * kBuckets + t];
 #pragma unroll
-      for (int u = 0; u < 32; ++u) {
-        if (s0 + u < o.spans) all += c[u];
-        if (s0 + u < static_cast<int>(blockIdx.x)) before += c[u];
-      }
+    for (int u = 0; u < 32; ++u) {
+      if (s0 + u < o.spans) all += c[u];
+      if (s0 + u < static_cast<int>(blockIdx.x)) before += c[u];
     }
   }
   uint32_t base = group_scan<16>(all, red);  // its barrier also ends the counting above
@@ -234,14 +235,55 @@ __global__ __launch_bounds__(1024) void embed_scatter_kernel(Order o) {
   });
 }
 
-// One workgroup per bucket: its positions ordered by token, and where each token's start.
+// One workgroup per bucket: its positions ordered by token, and where each token's start. With
+// kPick it first picks them out of all positions, in order, each wavefront out of an eighth.
+template <bool kPick>
 __global__ __launch_bounds__(512) void embed_order_kernel(Order o) {
   extern __shared__ uint32_t cursors[];  // [8][rows]
-  __shared__ uint32_t red[8];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  __shared__ uint32_t red[8], inside[8], below[8];
+  __shared__ uint32_t items[kPick ? kShort : 1];  // position, the token's low bits above 16
+  const int t = threadIdx.x, lane = t & 63, w = wave_index();
   const int rows = 1 << o.row_bits;
   uint32_t* const cur = cursors + w * rows;
-  const uint32_t b0 = o.bucket_at[blockIdx.x], b1 = o.bucket_at[blockIdx.x + 1];
+  const uint32_t first = static_cast<uint32_t>(blockIdx.x) << o.row_bits;  // the bucket's first token
+  uint32_t b0, b1;
+  if constexpr (kPick) {
+    constexpr int kBatches = kShort / 512;
+    const int64_t eighth = (o.n / 512 + 1) * 64, from = min(w * eighth, o.n), to = min(from + eighth, o.n);
+    uint32_t id[kBatches + 1];
+#pragma unroll
+    for (int u = 0; u <= kBatches; ++u) id[u] = static_cast<uint32_t>(token_of(o, from + u * 64 + lane, to));
+    uint32_t mine = 0, less = 0;
+#pragma unroll
+    for (int u = 0; u <= kBatches; ++u) {
+      mine += __popcll(__ballot(id[u] - first < static_cast<uint32_t>(rows)));
+      less += __popcll(__ballot(id[u] < first));
+    }
+    if (lane == 0) {
+      inside[w] = mine;
+      below[w] = less;
+    }
+    __syncthreads();
+    uint32_t at = 0;
+    b0 = 0, b1 = 0;
+    for (int k = 0; k < 8; ++k) {
+      if (k < w) at += inside[k];
+      b0 += below[k];
+      b1 += inside[k];
+    }
+    b1 += b0;
+#pragma unroll
+    for (int u = 0; u <= kBatches; ++u) {
+      const bool in = id[u] - first < static_cast<uint32_t>(rows);
+      const uint64_t m = __ballot(in);
+      if (in)
+        items[at + __popcll(m & ((uint64_t(1) << lane) - 1))] =
+            static_cast<uint32_t>(from + u * 64 + lane) | (id[u] - first) << 16;
+      at += __popcll(m);
+    }
+  } else {
+    b0 = o.bucket_at[blockIdx.x], b1 = o.bucket_at[blockIdx.x + 1];
+  }
   const uint32_t part = ((b1 - b0) / 512 + 1) * 64;  // 8 parts cover the bucket
   const uint32_t at = min(b0 + w * part, b1), end = min(at + part, b1);
   // f(i0, tokens, positions) for each batch in order
@@ -251,8 +293,13 @@ __global__ __launch_bounds__(512) void embed_order_kernel(Order o) {
 #pragma unroll
       for (int u = 0; u < kHeld; ++u) {
         const uint32_t i = min(i0 + u * 64 + lane, end - 1);
-        next_id[u] = o.item_id[i];
-        next_pos[u] = o.item_pos[i];
+        if constexpr (kPick) {
+          next_id[u] = first + (items[i - b0] >> 16);
+          next_pos[u] = items[i - b0] & 0xffff;
+        } else {
+          next_id[u] = o.item_id[i];
+          next_pos[u] = o.item_pos[i];
+        }
       }
     };
     if (at < end) fetch(at);
@@ -290,7 +337,7 @@ __global__ __launch_bounds__(512) void embed_order_kernel(Order o) {
     if (v < o.vocab) {
       o.start[v] = base;
       if (v == o.vocab - 1) o.start[o.vocab] = b1;
-      if (mine[j] > kLong) {
+      if (!kPick && mine[j] > kLong) {
         uint32_t* entry = o.long_list + 3 * atomicAdd(o.long_count, 1u);
         entry[0] = static_cast<uint32_t>(v);
         entry[1] = base;
@@ -396,12 +443,19 @@ __global__ __launch_bounds__(1024, 8) void embed_join_kernel(Order o, const T* g
                                                           const float* partial, T* gw) {
   __shared__ float sums[16][8][64];
   const int lane = threadIdx.x & 63;
-  const uint32_t w = wave_index(), lists = *o.long_count;
+  const uint32_t w = wave_index(), lists = o.pick ? (o.start[o.vocab] + kLong - 1) / kLong : *o.long_count;
   const int64_t c0 = static_cast<int64_t>(blockIdx.y) * kCols;
   for (uint32_t list = blockIdx.x; list < lists; list += gridDim.x) {
-    const uint32_t* entry = o.long_list + 3 * list;
-    const int64_t v = entry[0];
-    const uint32_t j0 = entry[1], j1 = entry[2];
+    int64_t v;
+    uint32_t j0, j1;
+    if (o.pick) {  // the list that holds position kLong * list and none of the multiples before
+      v = o.token[kLong * list];
+      j0 = o.start[v], j1 = o.start[v + 1];
+      if (j1 - j0 <= kLong || (j0 + kLong - 1) / kLong != list) continue;
+    } else {
+      const uint32_t* entry = o.long_list + 3 * list;
+      v = entry[0], j0 = entry[1], j1 = entry[2];
+    }
     const uint32_t tile = o.tile, t0 = (j0 + tile - 1) / tile, t1 = max(j1 / tile, t0);
     const uint32_t head = min(t0 * tile, j1), tail = max(t1 * tile, head);
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -492,6 +546,7 @@ int64_t lay_out(Order& o, float*& partial, void* ws, int64_t n, int64_t vocab, i
   // fp32 took 30 us in the sums and 9 in the join, with 16 23 and 5; 65,536 of 1536 in bf16 65 and 15, with
   // 32 71 and 16.
   o.tile = n <= 16384 ? 16 : 64;
+  o.pick = n <= kShort;
   char* base = static_cast<char*>(ws);
   int64_t used = 0;
   const auto take = [&](int64_t count) {
@@ -591,15 +646,21 @@ extern "C" int lema_embedding_grad(const void* gy, int32_t dtype, const int64_t*
   o.ids = ids;
   o.padding = padding;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t cols = (D + kCols - 1) / kCols, tiles = n / o.tile, longest = n / (kLong + 1);
+  const int64_t cols = (D + kCols - 1) / kCols, tiles = n / o.tile;
+  // long lists at most, or the places where one may be
+  const int64_t longest = o.pick && n > kLong ? (n + kLong - 1) / kLong : n / (kLong + 1);
   // a wavefront takes up to 3 slices: its chain of reads (start, positions, rows) is then shared
   const int64_t per = cols < 3 ? cols : 3, slices = (cols + per - 1) / per;
   const int64_t grid = ((tiles + vocab) * slices + 3) / 4;
   LEMA_REQUIRE(grid < (int64_t(1) << 24), "table [%lld, %lld] is too large", (long long)vocab,
                (long long)D);
-  if (o.spans > 1) embed_count_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
-  embed_scatter_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
-  embed_order_kernel<<<dim3(o.buckets), dim3(512), 8 * 4 << o.row_bits, st>>>(o);
+  if (o.pick) {
+    embed_order_kernel<true><<<dim3(o.buckets), dim3(512), 8 * 4 << o.row_bits, st>>>(o);
+  } else {
+    embed_count_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
+    embed_scatter_kernel<<<dim3(o.spans), dim3(1024), 0, st>>>(o);
+    embed_order_kernel<false><<<dim3(o.buckets), dim3(512), 8 * 4 << o.row_bits, st>>>(o);
+  }
   const RowKind kind = row_kind(dtype, D);
   // rows in, and the table's gradient out, past the Infinity Cache where they are larger than it: 65,536
   // rows of 1536 and a table of 50,304 in bf16 took 71 us, not 85 (of 1535: 71, not 82)

@@ -105,6 +105,23 @@ def test_gradient_of_the_largest(dev, dtype, n, V, D):
     check_grad(gw, ids, gy, V, 1.0)
 
 
+@pytest.mark.parametrize("n", [1, 33, 1024, 1025, 7167, 7168, 7169])
+@pytest.mark.parametrize("V", [1, 700, 50304, 1 << 20])
+def test_gradient_lengths_and_tables(dev, n, V):
+    """Around the lengths where the order is found another way, with every number of tokens a bucket,
+    frequent tokens at both ends of the table, ids outside it and a padding token."""
+    emb, g = table(dev, V, 24, torch.float32, seed=n, padding_idx=V // 2)
+    u = torch.rand(n, device=dev, generator=g, dtype=torch.float64)
+    ids = (V ** u).long().clamp_(1, V) - 1
+    ids[::3] = V - 1 - ids[::3]
+    ids[5::17] = V
+    ids[7::29] = -1
+    gy = torch.randn(n, 24, device=dev, generator=g)
+    (gw,) = torch.autograd.grad(embed(emb, ids), [emb.weight], gy)
+    check_grad(gw, ids, gy, V, 1.0, V // 2)
+    assert torch.equal(gw, torch.autograd.grad(embed(emb, ids), [emb.weight], gy)[0])
+
+
 @pytest.mark.parametrize("half", [520, 515])
 def test_rows_past_the_cache(dev, half):
     """Rows and a table of more than 256 MB: the columns as in calls of half of them."""
