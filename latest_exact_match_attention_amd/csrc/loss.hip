@@ -26,14 +26,16 @@ namespace {
 
 constexpr double kLog2e = 1.4426950408889634;
 
-// e^(k d) as 2^(d log2(e) k), the factor in two parts: its rounding alone, 1.3e-8 of it and the same
-// for every term, moved lp by 8e-8 on average, which adds up over an answer.
+// e^(k d), d <= 0, as 2^(d log2(e) k), the factor in two parts: its rounding alone, 1.3e-8 of it and the
+// same for every term, moved lp by 8e-8 on average, which adds up over an answer. hi is rounded down and
+// lo above 0, so that both products of d = -inf are -inf, whose power is 0: with a lo below 0, as the
+// nearest float leaves it at half of all temperatures, they would add up to NaN. `near` is that float.
 struct Scale {
-  float hi, lo;
+  float hi, lo, near;
   explicit Scale(float temperature) {
     const double k2 = kLog2e / temperature;
-    hi = static_cast<float>(k2);
-    lo = static_cast<float>(k2 - hi);
+    near = hi = static_cast<float>(k2);
+    while ((lo = static_cast<float>(k2 - hi)) <= 0.0f) hi = std::nextafter(hi, 0.0f);
   }
   __device__ __forceinline__ float exp(float d) const {
     return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo));
@@ -80,7 +82,7 @@ struct Running {
 };
 
 // Adds n logits to r. -FLT_MAX for the maximum of nothing, or of -inf alone, keeps
-// (-inf) - m = -inf, a zero, while a NaN stays one.
+// (-inf) - m = -inf, whose power is 0 at every temperature, while a NaN stays one.
 template <int N>
 __device__ __forceinline__ void add_logits(Running& r, const float (&x)[N], Scale k2) {
   float bm = x[0];
@@ -267,7 +269,7 @@ __global__ __launch_bounds__(kThreads, P > 7 ? 4 : 8) void policy_grad_kernel(
   for (int o = kWaves / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   // 2^(x k2 - m k2) in one FMA: the rounding of m k2 is the same in every term, so it leaves the
   // softmax alone, and the sum is set right for it below
-  const float mk = m * k2.hi;
+  const float mk = m * k2.near;
   const auto finish = [&](auto power, float off) {
     keep_packed(q);
     float s = power(xh) + power(xe);
@@ -324,9 +326,9 @@ __global__ __launch_bounds__(kThreads, P > 7 ? 4 : 8) void policy_grad_kernel(
     }
   };
   if (fabsf(mk) < 1048576.0f)  // its rounding is then below 2^-4
-    finish([&](float v) { return __builtin_amdgcn_exp2f(fmaf(v, k2.hi, -mk)); }, fmaf(m, k2.hi, -mk));
+    finish([&](float v) { return __builtin_amdgcn_exp2f(fmaf(v, k2.near, -mk)); }, fmaf(m, k2.near, -mk));
   else  // logits of any size, up to those whose product leaves fp32's range
-    finish([&](float v) { return __builtin_amdgcn_exp2f((v - m) * k2.hi); }, 0.0f);
+    finish([&](float v) { return __builtin_amdgcn_exp2f((v - m) * k2.near); }, 0.0f);
 }
 
 // Sum over the wavefront in 64 bits.
