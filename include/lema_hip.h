@@ -299,7 +299,8 @@ int lema_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t
 /* The logits' gradient where each row's lp has the gradient c = coef[r / per] * *scale0 * *scale1
  * (device scalars, NULL = 1): grad[r, j] = c / temperature * ([j = target[r]] - softmax[j]), in
  * fp32, rounded once; grad contiguous [rows, V]. Rows with c = 0 and rows that the mask leaves
- * out are not read: their gradient is zero. unit_done != 0: grad already holds the gradient for
+ * out are not read: their gradient is zero. Other rows whose target lies outside [0, V) get the
+ * gradient NaN. unit_done != 0: grad already holds the gradient for
  * *scale0 = 1 (lema_policy_loss wrote it) and is left as it is where *scale0 is 1. */
 int lema_token_logprobs_grad(const void* logits, int32_t dtype, int64_t rows, int64_t inner, int64_t V,
                              int64_t so, int64_t si, const int64_t* target, const uint8_t* mask,

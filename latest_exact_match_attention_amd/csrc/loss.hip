@@ -453,7 +453,8 @@ __global__ __launch_bounds__(1024) void preference_kernel(const double* lp, cons
 }
 
 // grad[row] = c k ([j = t] - e^(k (x_j - M)) / S), c = coef[row / per] * *scale0 * *scale1 (each
-// NULL: 1). grad is contiguous [rows, V]. Rows of c = 0 are not read. A gradient that is stored past
+// NULL: 1). grad is contiguous [rows, V]. Rows of c = 0 are not read; others whose target lies outside
+// [0, V) become NaN. A gradient that is stored past
 // the Infinity Cache leaves it to the logits, whose last rows the forward has just read: they come
 // first (8192 rows of 50,304 in bf16: 203 us, not 222).
 // unit_done: the forward has written the gradient for *scale0 = 1, which is then left as it is.
@@ -480,8 +481,9 @@ __global__ __launch_bounds__(kThreads) void logprob_grad_kernel(
       continue;
     }
     const float2 st = stats[row];
-    const float cs = c * st.y;
     const int64_t t = target[row];
+    if (t < 0 || t >= V) c = NAN;  // as the row's lp
+    const float cs = c * st.y;
     const T* x = logits + rows.at(row);
     const auto one = [&](int64_t j, float v) {
       const float e = k2.exp(v - st.x);

@@ -10,7 +10,8 @@ them). Logits are float32, float16 or bfloat16 on the device, [..., V] with a co
 (other layouts are copied; a slice like logits[:, :-1] is read in place); log-probabilities and
 losses are fp32. Only the logits are differentiable. A position that `mask` leaves out is not
 read: its log-probability and gradient are zero whatever its logits, target and other inputs
-hold. A counted position whose target lies outside [0, V) has the log-probability NaN. Logits of
+hold. A counted position whose target lies outside [0, V) has the log-probability NaN, and the
+gradient NaN unless its log-probability's gradient is zero. Logits of
 -inf have the probability 0; one whose distance to its row's maximum leaves fp32's range may too.
 """
 from __future__ import annotations

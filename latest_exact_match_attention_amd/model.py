@@ -307,7 +307,8 @@ class _CrossEntropySum(torch.autograd.Function):
 
 
 def cross_entropy_sum(logits: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
-    """Sum over rows of logsumexp(logits) - logits[y] (fp32), differentiable in the logits."""
+    """Sum over rows of logsumexp(logits) - logits[y] (fp32), differentiable in the logits. In bf16 on
+    the GPU a y outside the vocabulary makes the sum, and its row's gradient, NaN."""
     V = logits.shape[-1]
     if not (_fused(logits) and V % 8 == 0 and y.is_cuda):
         return F.cross_entropy(logits.float(), y, reduction="sum")

@@ -1,10 +1,11 @@
 """The losses where logits, targets and margins leave the ordinary: a vocabulary that is partly banned
-(-inf logits) at any temperature, against the same logits without the banned words."""
+(-inf logits) at any temperature, against the same logits in 64 bits; targets outside the vocabulary."""
 import pytest
 import torch
 from test_gpu_loss import E, TYPES, check_grad, exact, make
 
 from latest_exact_match_attention_amd.loss import policy_loss, preference_loss, token_logprobs
+from latest_exact_match_attention_amd.model import cross_entropy_sum
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +100,30 @@ def test_lowest_values(dev, dtype, temperature):
     assert bool(((lp.double() - want).abs() <= far)[:3].all()) and bool(lp[3:].isnan().all())
     (g,) = torch.autograd.grad(lp, [x], torch.ones_like(lp))
     assert bool(g[:3].isfinite().all()) and bool(g[3:].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [8, 1000, 50304])
+def test_targets_outside_the_vocabulary(dev, dtype, V):
+    """NaN where the log-probability or the loss is: a wrong target shows in the gradient too, not as
+    a descent on the whole row. A gradient of 0 of such a log-probability leaves its row alone."""
+    logits, targets, _ = make(dev, (4, 3), V, dtype, seed=V)
+    bad = torch.zeros(4, 3, dtype=torch.bool, device=dev)
+    bad[0, 1] = bad[1, 0] = bad[3, 2] = True
+    targets[0, 1], targets[1, 0], targets[3, 2] = -100, V, 1 << 32
+    logits.requires_grad_(True)
+    lp = token_logprobs(logits, targets)
+    assert torch.equal(lp.isnan(), bad)
+    (g,) = torch.autograd.grad(lp, [logits], torch.ones_like(lp), retain_graph=True)
+    assert bool(g[bad].isnan().all() and g[~bad].isfinite().all())
+    (g,) = torch.autograd.grad(torch.where(bad, 0.0, lp).sum(), [logits])
+    assert bool(g.isfinite().all()) and not g[bad].any() and bool(g[~bad].any())
+    if dtype == torch.bfloat16:
+        loss = cross_entropy_sum(logits.flatten(0, 1), targets)
+        (g,) = torch.autograd.grad(loss, [logits])
+        assert bool(loss.isnan() and g[bad].isnan().all() and g[~bad].isfinite().all())
+    z = torch.zeros(4, 3, device=dev)
+    r = policy_loss(logits, targets, z, z + 1, clip_high=1e3)
+    for up in (1.0, 2.0):
+        (g,) = torch.autograd.grad(up * r.loss, [logits], retain_graph=True)
+        assert bool(r.loss.isnan() and g[bad].isnan().all() and g[~bad].isfinite().all())
