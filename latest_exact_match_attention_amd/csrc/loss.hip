@@ -433,8 +433,10 @@ __global__ __launch_bounds__(1024) void preference_kernel(const double* lp, cons
       for (int i = 0; i < kWaves; ++i) d += sums[turn][team * kWaves + i];
       const float m = static_cast<float>(beta * d), e = expf(-fabsf(m));
       const float tail = log1pf(e), small = e / (1.0f + e), large = 1.0f / (1.0f + e);
-      // -log sigmoid(m) = tail + max(-m, 0);  sigmoid(|m|) = large, sigmoid(-|m|) = small
-      total += (1.0f - smooth) * (tail + fmaxf(-m, 0.0f)) + smooth * (tail + fmaxf(m, 0.0f));
+      // -log sigmoid(m) = tail + max(-m, 0);  sigmoid(|m|) = large, sigmoid(-|m|) = small. A part of
+      // weight 0 is left out: of an infinite margin (a banned word in an answer) it may be infinite
+      if (smooth < 1.0f) total += (1.0f - smooth) * (tail + fmaxf(-m, 0.0f));
+      if (smooth > 0.0f) total += smooth * (tail + fmaxf(m, 0.0f));
       if (m != m) total = m;
       // d term / d m = -(1 - smooth) sigmoid(-m) + smooth sigmoid(m)
       const float dm = smooth * (m > 0.0f ? large : small) - (1.0f - smooth) * (m > 0.0f ? small : large);

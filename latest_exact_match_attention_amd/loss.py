@@ -299,8 +299,9 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logprobs: t
     """The paired preference loss of 2 P answers of T tokens, logits [2 P, T, V]: answer p of the
     first P is preferred to answer P + p. With s an answer's sum of lp - ref_logprobs over its
     counted positions and m = beta (s_chosen - s_rejected), the mean over the pairs of
-    -(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m). ref_logprobs and mask
-    broadcast to the targets' shape [2 P, T]. The sums are formed in 64 bits."""
+    -(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m), where a part of weight 0
+    is left out. ref_logprobs and mask broadcast to the targets' shape [2 P, T]. The sums are formed
+    in 64 bits."""
     targets, mask = _check(logits, targets, mask, temperature)
     if targets.dim() != 2 or targets.shape[0] % 2 or targets.shape[0] == 0:
         raise ValueError(f"targets must be [2 P, T] with P >= 1, got {tuple(targets.shape)}")

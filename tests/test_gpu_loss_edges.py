@@ -1,5 +1,6 @@
 """The losses where logits, targets and margins leave the ordinary: a vocabulary that is partly banned
-(-inf logits) at any temperature, against the same logits in 64 bits; targets outside the vocabulary."""
+(-inf logits) at any temperature, against the same logits in 64 bits; targets outside the vocabulary;
+answers that cannot occur."""
 import pytest
 import torch
 from test_gpu_loss import E, TYPES, check_grad, exact, make
@@ -127,3 +128,39 @@ def test_targets_outside_the_vocabulary(dev, dtype, V):
     for up in (1.0, 2.0):
         (g,) = torch.autograd.grad(up * r.loss, [logits], retain_graph=True)
         assert bool(r.loss.isnan() and g[bad].isnan().all() and g[~bad].isfinite().all())
+
+
+@pytest.mark.parametrize("pairs", [1, 3, 20])
+@pytest.mark.parametrize("smooth", [0.0, 1.0, 0.25])
+@pytest.mark.parametrize("side", [0, 1])
+def test_infinite_margins(dev, pairs, smooth, side):
+    """An answer with a banned word is infinitely unlikely. Its pair costs nothing where the loss
+    asks for the other answer (and is infinite where it asks for this one at all), and the other
+    pairs keep their gradients."""
+    V, T = 40, 5
+    logits, targets, _ = make(dev, (2 * pairs, T), V, torch.float32, seed=7)
+    lp = torch.log_softmax(logits.double(), -1).gather(-1, targets[..., None])[..., 0]
+    row = side * pairs
+    logits[row, 2, targets[row, 2]] = -float("inf")
+    logits.requires_grad_(True)
+    ref = torch.full((2 * pairs, T), -3.0, device=dev)
+    r = preference_loss(logits, targets, ref, beta=0.5, label_smoothing=smooth)
+    (g,) = torch.autograd.grad(r.loss, [logits])
+    m = 0.5 * ((lp[:pairs] + 3).sum(1) - (lp[pairs:] + 3).sum(1))
+    m[0] = float("inf") if side else -float("inf")
+    ls = torch.nn.functional.logsigmoid
+    term = torch.zeros_like(m)
+    if smooth < 1:
+        term -= (1 - smooth) * ls(m)
+    if smooth > 0:
+        term -= smooth * ls(-m)
+    assert float(r.margins[0]) == float(m[0])
+    free = smooth == (0.0 if side else 1.0)
+    if free:
+        # margins of some tens are off by less than 64 E each, and a term by as much
+        assert abs(float(r.loss.detach()) - float(term.mean())) <= 64 * 64 * E
+    else:
+        assert float(r.loss.detach()) == float("inf")
+    assert bool(g.isfinite().all())
+    assert bool(g[row].any()) == (not free)
+    assert pairs == 1 or bool(g[1].any() and g[pairs + 1].any())
