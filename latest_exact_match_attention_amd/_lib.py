@@ -195,12 +195,18 @@ def dense(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous() if not t.is_neg() else t.resolve_neg().contiguous()
 
 
-def saved(t: torch.Tensor, like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+def placed(t: torch.Tensor, align: int) -> torch.Tensor:
+    """t, contiguous, at an address that is a multiple of `align` bytes: a slice of a larger tensor
+    may start at any element."""
+    return t if t.data_ptr() % align == 0 else t.clone()
+
+
+def saved(t: torch.Tensor, like: torch.Tensor, dtype: torch.dtype, align: int = 1) -> torch.Tensor:
     """A saved tensor as it was saved, on `like`'s device: a saved-tensor hook may bring it back in
-    another form."""
-    if t.dtype is dtype and t.device == like.device and t.is_contiguous() and not t.is_neg():
-        return t
-    return dense(t.to(device=like.device, dtype=dtype))
+    another form or at another address."""
+    if not (t.dtype is dtype and t.device == like.device and t.is_contiguous() and not t.is_neg()):
+        t = dense(t.to(device=like.device, dtype=dtype))
+    return placed(t, align)
 
 
 def needs_grad(*ts) -> bool:

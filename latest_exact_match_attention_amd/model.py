@@ -259,8 +259,8 @@ class _SwiGLUProduct(torch.autograd.Function):
     @staticmethod
     @_lib.once
     def backward(ctx, gy):
-        gy = _lib.dense(gy)
-        g, u = (_lib.saved(t, gy, gy.dtype) for t in ctx.saved_tensors)
+        gy = _lib.placed(_lib.dense(gy), 16)
+        g, u = (_lib.saved(t, gy, gy.dtype, 16) for t in ctx.saved_tensors)
         gg, gu = torch.empty_like(g), torch.empty_like(u)
         with _lib.device_of(gy):
             _lib.check(_lib.lib().lema_swiglu_grad_bf16(
