@@ -140,7 +140,7 @@ def _grad(ctx, like, coef, per, scale0, inv_n, grad=None):
     dev = like.device
     if logits.dtype is not ctx.dtype or logits.device != dev:
         logits = logits.to(device=dev, dtype=ctx.dtype)
-    targets, state = _lib.saved(targets, like, torch.long), _lib.saved(state, like, torch.float32)
+    targets, state = _lib.saved(targets, like, torch.long), _lib.saved(state, like, torch.float32, 8)
     mask = _lib.saved(mask, like, torch.bool) if mask is not None else None
     if ctx.logits is not None and ctx.logits[:2] == (logits.data_ptr(), logits.stride()):
         t, args = logits, ctx.logits[2]

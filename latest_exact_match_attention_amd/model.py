@@ -293,8 +293,8 @@ class _CrossEntropySum(torch.autograd.Function):
     @_lib.once
     def backward(ctx, g):
         logits, y, stats = ctx.saved_tensors
-        logits, y, stats = (_lib.saved(t, g, dt) for t, dt in
-                            ((logits, torch.bfloat16), (y, torch.long), (stats, torch.float32)))
+        logits, y, stats = (_lib.saved(t, g, dt, align) for t, dt, align in
+                            ((logits, torch.bfloat16, 1), (y, torch.long, 1), (stats, torch.float32, 8)))
         V = logits.shape[-1]
         rows = logits.numel() // V
         grad, coef = torch.empty_like(logits), -g.reshape(1)

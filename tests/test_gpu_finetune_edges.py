@@ -3,9 +3,17 @@ any address."""
 import pytest
 import torch
 
-from latest_exact_match_attention_amd.model import swiglu
+from latest_exact_match_attention_amd.loss import policy_loss, preference_loss, token_logprobs
+from latest_exact_match_attention_amd.model import cross_entropy_sum, embed, layer_norm, rms_norm, swiglu
 
 pytestmark = pytest.mark.gpu
+
+
+def moved(t, start=1):
+    """t as a slice of a larger tensor."""
+    flat = torch.empty(t.numel() + start, device=t.device, dtype=t.dtype)
+    flat[start:] = t.detach().reshape(-1)
+    return flat[start:].view(t.shape)
 
 
 @pytest.mark.parametrize("start", [1, 4, 8])
@@ -15,19 +23,38 @@ def test_swiglu_gradient_at_any_address(dev, start):
     torch.manual_seed(start)
     g, u, gy = (torch.randn(6, 40, device=dev).bfloat16() for _ in range(3))
     g.requires_grad_(True), u.requires_grad_(True)
-
-    def moved(t):
-        flat = torch.empty(t.numel() + start, device=dev, dtype=t.dtype)
-        flat[start:] = t.detach().reshape(-1)
-        return flat[start:].view(t.shape)
     want = torch.autograd.grad(swiglu(g, u), [g, u], gy)
-    got = torch.autograd.grad(swiglu(g, u), [g, u], moved(gy))
+    got = torch.autograd.grad(swiglu(g, u), [g, u], moved(gy, start))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     head = torch.zeros(start, device=dev, dtype=torch.bfloat16, requires_grad=True)
     joined = torch.cat([head, swiglu(g, u).reshape(-1)])
     got = torch.autograd.grad(joined, [g, u], torch.cat([head, gy.reshape(-1)]).detach())
     assert all(torch.equal(a, b) for a, b in zip(got, want))
-    with torch.autograd.graph.saved_tensors_hooks(moved, lambda t: t):
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: moved(t, start), lambda t: t):
         y = swiglu(g, u)
     got = torch.autograd.grad(y, [g, u], gy)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_saved_tensors_at_any_address(dev):
+    """Every operator's gradients with saved tensors that a hook brings back as slices."""
+    torch.manual_seed(3)
+    x = torch.randn(4, 3, 64, device=dev).bfloat16().requires_grad_(True)
+    t, z = torch.randint(0, 64, (4, 3), device=dev), torch.full((4, 3), -4.0, device=dev)
+    mask = torch.rand(4, 3, device=dev) < 0.7
+    norm, rms = (n(64, device=dev, dtype=torch.bfloat16) for n in (torch.nn.LayerNorm, torch.nn.RMSNorm))
+    emb = torch.nn.Embedding(70, 64, device=dev, dtype=torch.bfloat16)
+    cases = {
+        "logprobs": (lambda: token_logprobs(x, t, mask).sum(), [x]),
+        "policy": (lambda: 2.0 * policy_loss(x, t, z, z + 5, z, mask, kl_weight=0.1).loss, [x]),
+        "preference": (lambda: preference_loss(x, t, z, mask).loss, [x]),
+        "cross entropy": (lambda: cross_entropy_sum(x, t), [x]),
+        "layer norm": (lambda: layer_norm(x, norm)[0].square().sum(), [x, norm.weight, norm.bias]),
+        "rms norm": (lambda: rms_norm(x, rms, x * 2)[0].square().sum(), [x, rms.weight]),
+        "embed": (lambda: embed(emb, t, 3.0).square().sum(), [emb.weight])}
+    for name, (f, leaves) in cases.items():
+        want = torch.autograd.grad(f(), leaves)
+        with torch.autograd.graph.saved_tensors_hooks(moved, lambda s: s):
+            y = f()
+        got = torch.autograd.grad(y, leaves)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), name
