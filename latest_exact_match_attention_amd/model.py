@@ -632,6 +632,12 @@ class Attention(nn.Module):
         return self.merge(lema_hard(zq, zk, v))
 
 
+def _cached(x: torch.Tensor):
+    """What a forward with a cache runs in: the exchange has no gradient, and neither do the fused
+    bf16 launches around it."""
+    return torch.no_grad() if x.is_cuda and x.dtype is torch.bfloat16 else contextlib.nullcontext()
+
+
 class Block(nn.Module):
     def __init__(self, cfg: ModelConfig):
         super().__init__()
@@ -689,8 +695,7 @@ class Block(nn.Module):
     def forward(self, x, store=None):
         if store is not None:
             pre, post = self.seg or (self.gpu_pre, self.gpu_post)
-            # the exchange has no gradient, and neither do the fused bf16 launches around it
-            with torch.no_grad() if x.is_cuda and x.dtype is torch.bfloat16 else contextlib.nullcontext():
+            with _cached(x):
                 qc, kc, v = pre(x)
                 return post(x, store.exchange(qc, kc, v))
         h, x = rms_norm(x, self.norm2, self.attn(self.pre_attn(x)))
@@ -749,17 +754,19 @@ class Transformer(nn.Module):
             forward(next, cache=c)                    extending c
 
         With a cache, queries match keys from before this call too, so a sequence can be fed
-        in pieces; any chunking gives the one-shot result.
+        in pieces; any chunking gives the one-shot result. In bf16 on the GPU nothing of such a
+        call has a gradient, its logits neither.
         """
         if cache is not None and not (self.lema_layers()
                                       and all(a.hard for a in self.lema_layers())):
             raise ValueError("a cache needs an all-LEMA model in hard mode")
         x = self._embed(idx) if cache is None else self.tok_emb(idx)
-        for li, blk in enumerate(self.blocks):
-            x = blk(x, store=(cache.layer(li) if cache is not None else None))
-        if cache is not None:
-            cache.t += idx.shape[-1]
-        return linear(rms_norm(x, self.norm_f)[0], self.lm_head) if return_logits else None
+        with _cached(x) if cache is not None else contextlib.nullcontext():
+            for li, blk in enumerate(self.blocks):
+                x = blk(x, store=(cache.layer(li) if cache is not None else None))
+            if cache is not None:
+                cache.t += idx.shape[-1]
+            return linear(rms_norm(x, self.norm_f)[0], self.lm_head) if return_logits else None
 
     def _embed(self, idx):
         """The token rows: `embed`, whose gradient sorts the tokens, where one is wanted."""

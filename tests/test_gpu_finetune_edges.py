@@ -1,7 +1,8 @@
 """The model's functions in fine-tuning where a call leaves the ordinary: gradients and saved tensors at
-any address."""
+any address, caches."""
 import pytest
 import torch
+from test_gpu_finetune import build
 
 from latest_exact_match_attention_amd.loss import policy_loss, preference_loss, token_logprobs
 from latest_exact_match_attention_amd.model import cross_entropy_sum, embed, layer_norm, rms_norm, swiglu
@@ -58,3 +59,19 @@ def test_saved_tensors_at_any_address(dev):
             y = f()
         got = torch.autograd.grad(y, leaves)
         assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+
+
+@pytest.mark.parametrize("T", [1, 9, 40])
+def test_cached_logits_have_no_graph(dev, T):
+    """With a cache nothing has a gradient: no graph that ends at the final norm and head, whose
+    backward would fill two parameters and leave the others out without a word."""
+    model, _ = build(dev, 4)
+    idx = torch.randint(0, 200, (2, T), device=dev)
+    out = []
+    for ctx in (torch.no_grad(), torch.enable_grad()):
+        with ctx:
+            cache = model.new_cache("hbm", max_cache_len=64, batch=2)
+            out.append(model(idx, cache=cache))
+            assert not out[-1].requires_grad and cache.t == T
+    assert torch.equal(*out)
+    assert model(idx).requires_grad
