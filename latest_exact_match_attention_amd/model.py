@@ -124,10 +124,9 @@ class _Norm(torch.autograd.Function):
 def rms_norm(x: torch.Tensor, norm: nn.RMSNorm, d: torch.Tensor | None = None):
     """norm(x + d) and x + d (or norm(x), x when d is None), one pass in bf16; the gradients of
     x, d and the weight take one more and a sum over workgroups."""
-    if d is not None and not (_fused(x, d) and _fused(norm.weight)):
-        x, d = x + d, None
-    if not (_fused(x) and _fused(norm.weight) and x.shape[-1] % 8 == 0
-            and x.shape[-1] <= 4096):
+    if not (norm.weight is not None and _fused(x, norm.weight) and (d is None or _fused(d))
+            and x.shape[-1] % 8 == 0 and x.shape[-1] <= 4096):
+        x = x if d is None else x + d
         return norm(x), x
     eps = float(norm.eps if norm.eps is not None else torch.finfo(x.dtype).eps)
     return _norm(x, d, norm.weight, None, x.shape[-1], eps, False)

@@ -75,3 +75,23 @@ def test_cached_logits_have_no_graph(dev, T):
             assert not out[-1].requires_grad and cache.t == T
     assert torch.equal(*out)
     assert model(idx).requires_grad
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [20, 4104, 64])
+@pytest.mark.parametrize("affine", [True, False])
+def test_rms_norm_adds_the_addend(dev, dtype, D, affine):
+    """Also for rows that the kernel does not take, and without a weight. Both sides round s = x + d
+    once; the norm's factors and product in fp32 are 16 roundings off, then its own rounding."""
+    torch.manual_seed(D)
+    x, d = (torch.randn(5, D, device=dev).to(dtype).requires_grad_(True) for _ in range(2))
+    norm = torch.nn.RMSNorm(D, eps=1e-5, elementwise_affine=affine, device=dev, dtype=dtype)
+    h, s = rms_norm(x, norm, d)
+    assert torch.equal(s, x + d)
+    t = s.detach().double()
+    want = t * torch.rsqrt(t.square().mean(-1, keepdim=True) + 1e-5)
+    u = torch.finfo(dtype).eps / 2
+    # torch's own norm rounds the normalised row before the weight, too
+    assert bool(((h.double() - want).abs() <= (2 * u + 16 * 2.0 ** -24 + D * 2.0 ** -25) * want.abs()).all())
+    gx, gd = torch.autograd.grad(h.float().square().sum(), [x, d])
+    assert torch.equal(gx, gd) and bool(gx.isfinite().all())
