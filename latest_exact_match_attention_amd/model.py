@@ -124,7 +124,8 @@ class _Norm(torch.autograd.Function):
 def rms_norm(x: torch.Tensor, norm: nn.RMSNorm, d: torch.Tensor | None = None):
     """norm(x + d) and x + d (or norm(x), x when d is None), one pass in bf16; the gradients of
     x, d and the weight take one more and a sum over workgroups."""
-    if not (norm.weight is not None and _fused(x, norm.weight) and (d is None or _fused(d))
+    if not (norm.weight is not None and _fused(x, norm.weight) and norm.weight.shape == x.shape[-1:]
+            and (d is None or _fused(d) and d.shape == x.shape)
             and x.shape[-1] % 8 == 0 and x.shape[-1] <= 4096):
         x = x if d is None else x + d
         return norm(x), x
@@ -269,7 +270,7 @@ class _SwiGLUProduct(torch.autograd.Function):
 
 
 def swiglu(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
-    if not (_fused(g, u) and g.numel() % 8 == 0):
+    if not (_fused(g, u) and g.shape == u.shape and g.numel() % 8 == 0):
         return F.silu(g) * u
     return _SwiGLUProduct.apply(g, u) if _lib.needs_grad(g, u) else _swiglu_forward(g, u)
 
@@ -309,9 +310,9 @@ def cross_entropy_sum(logits: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
     """Sum over rows of logsumexp(logits) - logits[y] (fp32), differentiable in the logits. In bf16 on
     the GPU a y outside the vocabulary makes the sum, and its row's gradient, NaN."""
     V = logits.shape[-1]
-    if not (_fused(logits) and V % 8 == 0 and y.is_cuda):
+    rows = logits.numel() // V if V else 0
+    if not (_fused(logits) and V and V % 8 == 0 and y.device == logits.device and y.numel() == rows):
         return F.cross_entropy(logits.float(), y, reduction="sum")
-    rows = logits.numel() // V
     yy = y.reshape(-1).to(torch.int64).contiguous()
     if _lib.needs_grad(logits):
         return _CrossEntropySum.apply(logits, yy)
@@ -326,7 +327,8 @@ SKINNY_ROWS = 32  # products with at most this many token rows run on the skinny
 
 def _skinny(x: torch.Tensor, weight: torch.Tensor) -> bool:
     K = x.shape[-1]
-    return (_fused(x, weight) and K % 32 == 0 and 0 < x.numel() // K <= SKINNY_ROWS
+    return (_fused(x, weight) and K and K % 32 == 0 and weight.shape[-1] == K
+            and 0 < x.numel() // K <= SKINNY_ROWS
             and x.data_ptr() % 16 == 0 and weight.data_ptr() % 16 == 0)
 
 

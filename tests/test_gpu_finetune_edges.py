@@ -5,7 +5,7 @@ import torch
 from test_gpu_finetune import build
 
 from latest_exact_match_attention_amd.loss import policy_loss, preference_loss, token_logprobs
-from latest_exact_match_attention_amd.model import cross_entropy_sum, embed, layer_norm, rms_norm, swiglu
+from latest_exact_match_attention_amd.model import cross_entropy_sum, embed, layer_norm, linear, rms_norm, swiglu
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +95,32 @@ def test_rms_norm_adds_the_addend(dev, dtype, D, affine):
     assert bool(((h.double() - want).abs() <= (2 * u + 16 * 2.0 ** -24 + D * 2.0 ** -25) * want.abs()).all())
     gx, gd = torch.autograd.grad(h.float().square().sum(), [x, d])
     assert torch.equal(gx, gd) and bool(gx.isfinite().all())
+
+
+def test_shapes_that_do_not_match(dev):
+    """What torch broadcasts is broadcast, and what it refuses is refused: no kernel reads or writes
+    by the first argument's size alone."""
+    torch.manual_seed(5)
+    x = torch.randn(6, 64, device=dev).bfloat16().requires_grad_(True)
+    d = torch.randn(64, device=dev).bfloat16().requires_grad_(True)
+    norm = torch.nn.RMSNorm(64, device=dev, dtype=torch.bfloat16)
+    h, s = rms_norm(x, norm, d)
+    assert torch.equal(s, x + d) and torch.equal(h, norm(x + d))
+    assert torch.autograd.grad(h.float().square().sum(), [d])[0].shape == d.shape
+    wide = torch.nn.RMSNorm((6, 64), device=dev, dtype=torch.bfloat16)
+    assert torch.equal(rms_norm(x, wide)[0], wide(x))
+    with pytest.raises(RuntimeError):
+        rms_norm(x, torch.nn.RMSNorm(32, device=dev, dtype=torch.bfloat16))
+    y = swiglu(x, d)
+    assert torch.equal(y, torch.nn.functional.silu(x) * d)
+    assert torch.autograd.grad(y.float().sum(), [d])[0].shape == d.shape
+    with pytest.raises(RuntimeError):
+        swiglu(x, d[:32])
+    t = torch.zeros(6, dtype=torch.long, device=dev)
+    for wrong in (t[:4], torch.cat([t, t])):
+        with pytest.raises(ValueError):
+            cross_entropy_sum(x, wrong)
+    with pytest.raises(RuntimeError):
+        cross_entropy_sum(x, t.cpu())
+    with pytest.raises(RuntimeError):
+        linear(x, torch.nn.Linear(96, 8, bias=False, device=dev, dtype=torch.bfloat16))
