@@ -208,14 +208,35 @@ class _Embed(torch.autograd.Function):
         return gw, None, None, None
 
 
+_MODULES = torch.nn.modules.module
+
+
+def _plain(emb: nn.Module) -> bool:
+    """Whether a call of emb does nothing but look rows up in its table: an nn.Embedding itself, with
+    no hooks and no forward of its own. torch has no public names for these; one that is missing
+    counts as a hook."""
+    try:
+        return (type(emb) is nn.Embedding and "forward" not in emb.__dict__
+                and not (emb._forward_hooks or emb._forward_pre_hooks or emb._backward_hooks
+                         or emb._backward_pre_hooks or _MODULES._global_forward_hooks
+                         or _MODULES._global_forward_pre_hooks or _MODULES._global_backward_hooks
+                         or _MODULES._global_backward_pre_hooks))
+    except AttributeError:
+        return False
+
+
 def embed(emb: nn.Embedding, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """emb(ids) * scale, rounded once, in float32, float16 or bfloat16. The ids must lie in
-    [0, vocab): an id outside it gives a zero row and no gradient, where nn.Embedding raises.
+    [0, vocab): on the GPU one outside it gives a zero row and no gradient.
 
     Differentiable in the table (`padding_idx` gets a zero gradient): the gradient adds up each
-    token's rows in a fixed order, in fp32. A table that nn.Embedding renormalises (max_norm), a
-    sparse gradient or one scaled by frequency, a table of more than 2^20 rows that wants a
-    gradient, and CPU tensors take the torch operations."""
+    token's rows in a fixed order, in fp32. A module with hooks or with a forward of its own is
+    called. So is one that renormalises its table (max_norm), wants a sparse gradient or one scaled
+    by frequency, or a gradient of more than 2^20 rows, or lies on the CPU; the scale's product is
+    then an operation of its own."""
+    if not _plain(emb):
+        y = emb(ids)
+        return y if scale == 1.0 else y * scale
     w = emb.weight
     grad = _lib.needs_grad(w)
     if not (w.is_cuda and ids.device == w.device and w.dtype in _lib.DTYPE_CODE and w.is_contiguous()
@@ -224,7 +245,8 @@ def embed(emb: nn.Embedding, ids: torch.Tensor, scale: float = 1.0) -> torch.Ten
             and not (grad and (emb.sparse or emb.scale_grad_by_freq or w.shape[0] > 1 << 20))):
         y = emb(ids)
         return y if scale == 1.0 else y * scale
-    ids = ids.long().contiguous()
+    if ids.dtype is not torch.long or not ids.is_contiguous():
+        ids = ids.long().contiguous()
     if grad:
         return _Embed.apply(w, ids, float(scale), -1 if emb.padding_idx is None else emb.padding_idx)
     return _embed_forward(w, ids, float(scale))
@@ -771,7 +793,8 @@ class Transformer(nn.Module):
 
     def _embed(self, idx):
         """The token rows: `embed`, whose gradient sorts the tokens, where one is wanted."""
-        return embed(self.tok_emb, idx) if _lib.needs_grad(self.tok_emb.weight) else self.tok_emb(idx)
+        emb = self.tok_emb
+        return embed(emb, idx) if _plain(emb) and _lib.needs_grad(emb.weight) else emb(idx)
 
     def hidden(self, idx):
         """The final normalised hidden states (the input of lm_head), without a cache."""

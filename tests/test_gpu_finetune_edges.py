@@ -1,5 +1,5 @@
 """The model's functions in fine-tuning where a call leaves the ordinary: gradients and saved tensors at
-any address, caches."""
+any address, caches, shapes, modules that do more than they are named for."""
 import pytest
 import torch
 from test_gpu_finetune import build
@@ -124,3 +124,73 @@ def test_shapes_that_do_not_match(dev):
         cross_entropy_sum(x, t.cpu())
     with pytest.raises(RuntimeError):
         linear(x, torch.nn.Linear(96, 8, bias=False, device=dev, dtype=torch.bfloat16))
+
+
+class Doubled(torch.nn.Embedding):
+    def forward(self, ids):
+        return 2 * super().forward(ids)
+
+
+class Wrapped(torch.nn.Module):
+    """An embedding without a table of its own."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, ids):
+        return 2 * self.inner(ids)
+
+
+def doubled_by(kind, emb):
+    """emb, or what stands for it, with rows twice as large, and what takes that back."""
+    if kind == "subclass":
+        return Doubled(*emb.weight.shape, _weight=emb.weight.detach().clone()), lambda: None
+    if kind == "wrapper":
+        return Wrapped(emb), lambda: None
+    if kind == "own forward":
+        plain = emb.forward
+        emb.forward = lambda ids: 2 * plain(ids)
+        return emb, lambda: None
+    if kind == "hook":
+        return emb, emb.register_forward_hook(lambda m, i, o: 2 * o).remove
+    if kind == "pre-hook":                       # the other half of the table holds the doubled rows
+        with torch.no_grad():
+            emb.weight[128:] = 2 * emb.weight[:128]
+        return emb, emb.register_forward_pre_hook(lambda m, i: (i[0] + 128,)).remove
+    every = torch.nn.modules.module.register_module_forward_hook
+    return emb, every(lambda m, i, o: 2 * o if m is emb else None).remove
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["subclass", "wrapper", "own forward", "hook", "pre-hook", "global hook"])
+@pytest.mark.parametrize("B,T", [(2, 9), (4, 600)])
+def test_embedding_modules_are_called(dev, dtype, kind, B, T):
+    """Hooks and forwards of an embedding run in training as they do without gradients, in the
+    function and in the model."""
+    model, _ = build(dev, 6)
+    model.to(dtype)
+    idx = torch.randint(0, 128, (B, T), device=dev)
+    rows = model.tok_emb.weight.detach()[idx]
+    model.tok_emb, undo = doubled_by(kind, model.tok_emb)
+    try:
+        assert torch.equal(embed(model.tok_emb, idx), 2 * rows)
+        assert torch.equal(embed(model.tok_emb, idx, 3.0), 2 * rows * 3.0)
+        with torch.no_grad():
+            assert torch.equal(embed(model.tok_emb, idx), 2 * rows)
+        seen = []
+        handle = model.blocks[0].register_forward_pre_hook(lambda m, i: seen.append(i[0].detach()))
+        assert model(idx).requires_grad and model.hidden(idx).requires_grad
+        handle.remove()
+        assert len(seen) == 2 and all(torch.equal(x, 2 * rows) for x in seen)
+    finally:
+        undo()
+
+
+def test_backward_hooks_of_an_embedding(dev):
+    model, _ = build(dev, 7)
+    idx = torch.randint(0, 200, (4, 600), device=dev)
+    seen = []
+    model.tok_emb.register_full_backward_hook(lambda m, gi, go: seen.append(go[0].shape))
+    model(idx).float().square().sum().backward()
+    assert seen == [(4, 600, 64)]
