@@ -43,7 +43,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import _lib
-from .attention import code_dtype_for, lema_from_codes, lema_hard, pack_codes
+from .attention import _unwatched, code_dtype_for, lema_from_codes, lema_hard, pack_codes
 
 __all__ = ["ModelConfig", "SwiGLU", "Attention", "Block", "Transformer", "lm_loss", "rms_norm",
            "layer_norm", "embed", "argmax_into", "load_trained",
@@ -183,6 +183,25 @@ def _embed_forward(w, ids, scale):
     return out
 
 
+def _embed_backward(ctx, gy):
+    V, D, scale, padding, n = ctx.table
+    ids = _lib.saved(ctx.saved_tensors[0], gy, torch.long)
+    if type(gy) is not torch.Tensor or torch.is_grad_enabled() or not _unwatched(gy):
+        # a graph of the backward, batched or otherwise wrapped gradients: operations that compose
+        keep = (ids >= 0) & (ids < V) & (ids != padding)
+        rows = torch.where(keep[..., None], gy.float() * scale, 0.0).reshape(-1, D)
+        gw = torch.index_add(rows.new_zeros(V, D), 0, torch.where(keep, ids, 0).reshape(-1), rows)
+        return gw.to(gy.dtype), None, None, None
+    gy = _lib.dense(gy)
+    gw = gy.new_empty(V, D)
+    ws = gy.new_empty(n, dtype=torch.uint8)
+    with _lib.device_of(gy):
+        _lib.check(_lib.lib().lema_embedding_grad(
+            gy.data_ptr(), _lib.DTYPE_CODE[gy.dtype], ids.data_ptr(), ids.numel(), V, D, scale, padding,
+            gw.data_ptr(), ws.data_ptr(), n, _lib.stream_of(gy)))
+    return gw, None, None, None
+
+
 class _Embed(torch.autograd.Function):
     """The lookup, and the table's gradient by sorted tokens (its sums have a fixed order)."""
 
@@ -193,19 +212,12 @@ class _Embed(torch.autograd.Function):
         ctx.table = V, D, scale, padding, _lib.lib().lema_embedding_grad_workspace_bytes(ids.numel(), V, D)
         return _embed_forward(w, ids, scale)
 
-    @staticmethod
-    @_lib.once
-    def backward(ctx, gy):
-        V, D, scale, padding, n = ctx.table
-        gy = _lib.dense(gy)
-        ids = _lib.saved(ctx.saved_tensors[0], gy, torch.long)
-        gw = gy.new_empty(V, D)
-        ws = gy.new_empty(n, dtype=torch.uint8)
-        with _lib.device_of(gy):
-            _lib.check(_lib.lib().lema_embedding_grad(
-                gy.data_ptr(), _lib.DTYPE_CODE[gy.dtype], ids.data_ptr(), ids.numel(), V, D, scale, padding,
-                gw.data_ptr(), ws.data_ptr(), n, _lib.stream_of(gy)))
-        return gw, None, None, None
+    backward = staticmethod(_lib.once(_embed_backward))
+
+
+class _ModelEmbed(_Embed):
+    """The same in a model, whose exact op and fp32 operations have gradients of gradients."""
+    backward = staticmethod(_embed_backward)
 
 
 _MODULES = torch.nn.modules.module
@@ -234,6 +246,11 @@ def embed(emb: nn.Embedding, ids: torch.Tensor, scale: float = 1.0) -> torch.Ten
     called. So is one that renormalises its table (max_norm), wants a sparse gradient or one scaled
     by frequency, or a gradient of more than 2^20 rows, or lies on the CPU; the scale's product is
     then an operation of its own."""
+    return _embed(emb, ids, scale, _Embed)
+
+
+def _embed(emb, ids, scale, function):
+    """embed, with the autograd Function that records it."""
     if not _plain(emb):
         y = emb(ids)
         return y if scale == 1.0 else y * scale
@@ -248,7 +265,7 @@ def embed(emb: nn.Embedding, ids: torch.Tensor, scale: float = 1.0) -> torch.Ten
     if ids.dtype is not torch.long or not ids.is_contiguous():
         ids = ids.long().contiguous()
     if grad:
-        return _Embed.apply(w, ids, float(scale), -1 if emb.padding_idx is None else emb.padding_idx)
+        return function.apply(w, ids, float(scale), -1 if emb.padding_idx is None else emb.padding_idx)
     return _embed_forward(w, ids, float(scale))
 
 
@@ -794,7 +811,7 @@ class Transformer(nn.Module):
     def _embed(self, idx):
         """The token rows: `embed`, whose gradient sorts the tokens, where one is wanted."""
         emb = self.tok_emb
-        return embed(emb, idx) if _plain(emb) and _lib.needs_grad(emb.weight) else emb(idx)
+        return _embed(emb, idx, 1.0, _ModelEmbed) if _plain(emb) and _lib.needs_grad(emb.weight) else emb(idx)
 
     def hidden(self, idx):
         """The final normalised hidden states (the input of lm_head), without a cache."""

@@ -194,3 +194,56 @@ def test_backward_hooks_of_an_embedding(dev):
     model.tok_emb.register_full_backward_hook(lambda m, gi, go: seen.append(go[0].shape))
     model(idx).float().square().sum().backward()
     assert seen == [(4, 600, 64)]
+
+
+def test_embedding_gradients_compose(dev):
+    """A graph of the backward of a model in fp32: as from the embedding module's own gradient, which
+    a hook that does nothing brings about. The two add a token's rows up in other orders: some 40
+    of them, each sum off by 40 2^-24 of its terms, whose sum a cancellation leaves a fifth of."""
+    model, _ = build(dev, 8)
+    model.float()
+    idx = torch.randint(0, 200, (4, 600), device=dev)
+    w = model.tok_emb.weight
+    v = torch.randn(w.shape, device=dev, generator=torch.Generator(dev).manual_seed(1))
+
+    def products():
+        y = model.hidden(idx)
+        (g,) = torch.autograd.grad(y.square().sum(-1).sqrt().mean(), [w], create_graph=True)
+        (hv,) = torch.autograd.grad((g * v).sum(), [w])
+        return g.detach(), hv
+    got = products()
+    handle = model.tok_emb.register_forward_hook(lambda m, i, o: None)
+    want = products()
+    handle.remove()
+    for a, b in zip(got, want):
+        assert float((a - b).norm()) <= 2 * 5 * 40 * 2.0 ** -24 * float(b.norm()) and bool(b.any())
+
+
+@pytest.mark.parametrize("dtype,scale,pad", [(torch.float32, 1.0, None), (torch.bfloat16, 3.0, 5)])
+def test_embedding_gradients_in_batches(dev, dtype, scale, pad):
+    """Each as the gradient alone."""
+    torch.manual_seed(9)
+    ids = torch.randint(-3, 203, (300,), device=dev)
+    emb = torch.nn.Embedding(200, 24, padding_idx=pad, device=dev, dtype=dtype)
+    y = embed(emb, ids, scale)
+    gy = torch.randn(3, *y.shape, device=dev).to(dtype)
+    (many,) = torch.autograd.grad(y, [emb.weight], gy, is_grads_batched=True, retain_graph=True)
+    m, u = int(torch.bincount(ids.clamp_min(0)).max()), torch.finfo(dtype).eps / 2
+    for k in range(3):
+        (one,) = torch.autograd.grad(y, [emb.weight], gy[k], retain_graph=True)
+        # each side sums up to m products of at most scale max |gy| in fp32, and rounds once
+        tol = 2 * m * 2.0 ** -24 * m * scale * float(gy.abs().max())
+        assert bool(((many[k].double() - one.double()).abs() <= 2 * u * one.double().abs() + 2 * tol).all())
+        assert pad is None or not many[k][pad].any()
+
+
+@pytest.mark.parametrize("name", ["logprobs", "norm", "swiglu"])
+def test_batched_gradients_are_refused(dev, name):
+    """The other operators' gradients come one at a time, and say so."""
+    x = torch.randn(4, 64, device=dev).bfloat16().requires_grad_(True)
+    norm = torch.nn.LayerNorm(64, device=dev, dtype=torch.bfloat16)
+    f = {"logprobs": lambda: token_logprobs(x, torch.zeros(4, dtype=torch.long, device=dev)),
+         "norm": lambda: layer_norm(x, norm)[0], "swiglu": lambda: swiglu(x, x)}[name]
+    y = f()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, [x], torch.ones(2, *y.shape, device=dev, dtype=y.dtype), is_grads_batched=True)
