@@ -220,6 +220,12 @@ class _ModelEmbed(_Embed):
     backward = staticmethod(_embed_backward)
 
 
+# Positions from which a model's lookup takes the gradient by sorted tokens. A lookup with its
+# gradient in torch's two operations took 88 to 223 us at 2048 positions, by table (256 x 64 to
+# 50,304 x 1536) and tokens (even, Zipf, all the same), and 83 to 88 so; 1024 took 51 to 123 and 82 to 94,
+# 200 took 48 to 64 and 81 to 87, of which Python's part of autograd is two thirds.
+SORTED_GRAD_MIN = 2048
+
 _MODULES = torch.nn.modules.module
 
 
@@ -794,7 +800,8 @@ class Transformer(nn.Module):
             forward(next, cache=c)                    extending c
 
         With a cache, queries match keys from before this call too, so a sequence can be fed
-        in pieces; any chunking gives the one-shot result. In bf16 on the GPU nothing of such a
+        in pieces; any chunking gives the one-shot result. Tokens must lie in [0, vocab_size);
+        on the GPU they are not checked. In bf16 on the GPU nothing of such a
         call has a gradient, its logits neither.
         """
         if cache is not None and not (self.lema_layers()
@@ -809,9 +816,11 @@ class Transformer(nn.Module):
             return linear(rms_norm(x, self.norm_f)[0], self.lm_head) if return_logits else None
 
     def _embed(self, idx):
-        """The token rows: `embed`, whose gradient sorts the tokens, where one is wanted."""
+        """The token rows: `embed`, whose gradient sorts the tokens, where one of many is wanted."""
         emb = self.tok_emb
-        return _embed(emb, idx, 1.0, _ModelEmbed) if _plain(emb) and _lib.needs_grad(emb.weight) else emb(idx)
+        if idx.numel() >= SORTED_GRAD_MIN and _plain(emb) and _lib.needs_grad(emb.weight):
+            return _embed(emb, idx, 1.0, _ModelEmbed)
+        return emb(idx)
 
     def hidden(self, idx):
         """The final normalised hidden states (the input of lm_head), without a cache."""

@@ -247,3 +247,18 @@ def test_batched_gradients_are_refused(dev, name):
     y = f()
     with pytest.raises(RuntimeError):
         torch.autograd.grad(y, [x], torch.ones(2, *y.shape, device=dev, dtype=y.dtype), is_grads_batched=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_short_lookups_keep_torchs_gradient(dev, dtype):
+    """A model's lookup with its gradient is not slower than torch's two operations: those are kept
+    below 2048 positions, whose gradient the sort makes no faster. Either gives the same rows."""
+    model, _ = build(dev, 10)
+    model.to(dtype)
+    for B, T, sorts in ((1, 1, False), (3, 200, False), (1, 2047, False), (4, 512, True), (2, 1500, True)):
+        idx = torch.randint(0, 200, (B, T), device=dev)
+        y = model._embed(idx)
+        assert ("ModelEmbed" in y.grad_fn.name()) == sorts
+        assert torch.equal(y, model.tok_emb.weight[idx])
+        with torch.no_grad():
+            assert model._embed(idx).grad_fn is None
