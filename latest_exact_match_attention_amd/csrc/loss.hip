@@ -570,6 +570,8 @@ int grad_launch(const void* logits, int32_t dtype, int64_t rows, int64_t inner, 
 bool one_pass(int32_t dtype, int64_t V) { return V * dtype_size(dtype) <= 16 * 1024 * 16; }
 
 // Calls f with the threads of a row's workgroup and the pieces each holds, as compile-time constants.
+// Up to 7 pieces leave a CU two workgroups of 1024, 10 and 16 one: 6144 rows of bf16 ran at 4.9 to 5.3 TB/s
+// up to 57,344 logits, at 4.7 to 4.8 from 65,536 to 131,072, and read twice, at 3.8, beyond.
 template <typename T, typename F>
 inline void for_pieces(int64_t V, F f) {
   using std::integral_constant;

@@ -64,7 +64,8 @@ __global__ __launch_bounds__(256) void swiglu_kernel(const u32x4* gate, const u3
 }
 
 // y = s u with s = g sig, sig = 1 / (1 + e^-g):  gu = gy s,  gg = gy u sig (1 + g (1 - sig)), in
-// fp32 with one rounding each; a piece of each input per thread and trip.
+// fp32 with one rounding each; a piece of each input per thread and trip. Bound by HBM: [65536, 6144]
+// took 748 us, 5.4 TB/s of five tensors, where a copy of 512 MiB ran at 5.8 to 5.9.
 __global__ __launch_bounds__(256) void swiglu_grad_kernel(const u32x4* gate, const u32x4* up,
                                                           const u32x4* gy, u32x4* g_gate, u32x4* g_up,
                                                           int64_t n8) {

@@ -800,9 +800,9 @@ class Transformer(nn.Module):
             forward(next, cache=c)                    extending c
 
         With a cache, queries match keys from before this call too, so a sequence can be fed
-        in pieces; any chunking gives the one-shot result. Tokens must lie in [0, vocab_size);
-        on the GPU they are not checked. In bf16 on the GPU nothing of such a
-        call has a gradient, its logits neither.
+        in pieces; any chunking gives the one-shot result. In bf16 on the GPU nothing of a call
+        with a cache has a gradient, its logits neither. Tokens must lie in [0, vocab_size); on the
+        GPU they are not checked.
         """
         if cache is not None and not (self.lema_layers()
                                       and all(a.hard for a in self.lema_layers())):
