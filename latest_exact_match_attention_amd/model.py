@@ -54,8 +54,10 @@ __all__ = ["ModelConfig", "SwiGLU", "Attention", "Block", "Transformer", "lm_los
 # run as one HIP kernel each (liblema_hip.so); other dtypes and devices use the torch ops.
 
 def _fused(*ts: torch.Tensor) -> bool:
+    """Whether the kernels take the tensors as they lie: bf16 on the GPU, contiguous, from a 16-byte
+    boundary on (a slice, or a parameter in a flat buffer, may start elsewhere)."""
     for t in ts:
-        if not (t.is_cuda and t.dtype is torch.bfloat16 and t.is_contiguous()):
+        if not (t.is_cuda and t.dtype is torch.bfloat16 and t.is_contiguous() and t.data_ptr() % 16 == 0):
             return False
     return True
 

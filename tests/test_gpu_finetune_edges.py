@@ -296,3 +296,35 @@ def test_step_of_a_batch(dev, kind):
         else:
             off = float((g.double() - r).norm() / r.norm())
             assert off <= 4 * 10 * 2.0 ** -9, (n, off)
+
+
+def test_inputs_at_any_address(dev):
+    """Activations and weights that are slices of larger tensors, with their gradients: torch's
+    operations take what the fused kernels do not."""
+    torch.manual_seed(11)
+    x, d, u = (moved(torch.randn(40, 64, device=dev).bfloat16()).requires_grad_(True) for _ in range(3))
+    norm = torch.nn.RMSNorm(64, device=dev, dtype=torch.bfloat16)
+    norm.weight = torch.nn.Parameter(moved(torch.rand(64, device=dev).bfloat16()))
+    t = torch.randint(0, 64, (40,), device=dev)
+    h, s = rms_norm(x, norm, d)
+    assert torch.equal(s, x + d) and torch.equal(h, norm(x + d))
+    assert torch.equal(swiglu(x, u), torch.nn.functional.silu(x) * u)
+    loss = cross_entropy_sum(x, t)
+    assert torch.equal(loss, torch.nn.functional.cross_entropy(x.float(), t, reduction="sum"))
+    total = h.float().square().sum() + swiglu(x, u).float().sum() + loss
+    assert all(bool(g.isfinite().all()) for g in torch.autograd.grad(total, [x, d, u, norm.weight]))
+    # a model whose parameters lie in one flat buffer
+    model, _ = build(dev, 12)
+    idx = torch.randint(0, 200, (3, 40), device=dev)
+    with torch.no_grad():
+        want = model(idx)
+        flat = torch.empty(1 + sum(p.numel() + 1 for p in model.parameters()), device=dev, dtype=torch.bfloat16)
+        at = 1
+        for p in model.parameters():
+            flat[at:at + p.numel()] = p.reshape(-1)
+            p.data = flat[at:at + p.numel()].view(p.shape)
+            at += p.numel() + 1
+        got = model(idx)
+    # other kernels: a few roundings of bf16 a layer, which may turn a code's sign
+    assert got.shape == want.shape and bool(got.isfinite().all())
+    assert float(torch.autograd.grad(model(idx).float().square().mean(), [model.lm_head.weight])[0].norm()) > 0
