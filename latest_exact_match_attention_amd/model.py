@@ -225,7 +225,7 @@ class _ModelEmbed(_Embed):
 # Positions from which a model's lookup takes the gradient by sorted tokens. A lookup with its
 # gradient in torch's two operations took 88 to 223 us at 2048 positions, by table (256 x 64 to
 # 50,304 x 1536) and tokens (even, Zipf, all the same), and 83 to 88 so; 1024 took 51 to 123 and 82 to 94,
-# 200 took 48 to 64 and 81 to 87, of which Python's part of autograd is two thirds.
+# 200 took 48 to 64 and 81 to 87, most of it the host's.
 SORTED_GRAD_MIN = 2048
 
 _MODULES = torch.nn.modules.module
@@ -359,6 +359,8 @@ def cross_entropy_sum(logits: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
     V = logits.shape[-1]
     rows = logits.numel() // V if V else 0
     if not (_fused(logits) and V and V % 8 == 0 and y.device == logits.device and y.numel() == rows):
+        if V and y.shape == logits.shape[:-1]:  # the vocabulary is the last dim here, the second one there
+            logits, y = logits.reshape(rows, V), y.reshape(rows)
         return F.cross_entropy(logits.float(), y, reduction="sum")
     yy = y.reshape(-1).to(torch.int64).contiguous()
     if _lib.needs_grad(logits):

@@ -328,3 +328,16 @@ def test_inputs_at_any_address(dev):
     # other kernels: a few roundings of bf16 a layer, which may turn a code's sign
     assert got.shape == want.shape and bool(got.isfinite().all())
     assert float(torch.autograd.grad(model(idx).float().square().mean(), [model.lm_head.weight])[0].norm()) > 0
+
+
+@pytest.mark.parametrize("shape", [(5, 3, 20), (4, 24, 24), (20,), (6, 24)])
+def test_cross_entropy_over_the_last_dim(dev, shape):
+    """Whatever the type, length and address of the rows, the vocabulary is the last dim."""
+    torch.manual_seed(13)
+    x = torch.randn(*shape, device=dev)
+    y = torch.randint(0, shape[-1], shape[:-1], device=dev)
+    for t in (x, x.bfloat16(), moved(x.bfloat16())):
+        want = -torch.log_softmax(t.double(), -1).gather(-1, y[..., None]).sum()
+        got = cross_entropy_sum(t, y)
+        # rows of some 3 each, added up in fp32: 40 roundings of at most the sum
+        assert abs(float(got) - float(want)) <= 40 * 2.0 ** -24 * float(want)
