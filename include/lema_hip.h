@@ -270,12 +270,23 @@ int lema_fp8_matmul(const void* a, const void* sa, int64_t lds, const void* w, c
                     const void* w2, const void* sw2, int32_t dtype, int64_t M, int64_t N, int64_t K,
                     void* out, void* ws, int64_t ws_bytes, void* stream);
 
-/* The same of at most 32 rows of x [M, K] (bf16 or fp16, row stride ldx, any element's address), which
+/* The same with out in fp32, every product exact and the sums in fp32. */
+int64_t lema_fp8_matmul_f32_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t gated);
+int lema_fp8_matmul_f32(const void* a, const void* sa, int64_t lds, const void* w, const void* sw,
+                        const void* w2, const void* sw2, int64_t M, int64_t N, int64_t K, void* out, void* ws,
+                        int64_t ws_bytes, void* stream);
+
+/* lema_fp8_matmul of at most 32 rows of x [M, K] (bf16 or fp16, row stride ldx, any element's address), which
  * the launch quantizes itself: bit for bit the values of lema_fp8_quantize. residual (NULL or [M, N] of
  * the same type) is added to the rounded product. */
 int lema_fp8_linear(const void* x, int32_t dtype, int64_t ldx, const void* w, const void* sw, const void* w2,
                     const void* sw2, const void* residual, int64_t M, int64_t N, int64_t K, void* out,
                     void* stream);
+
+/* The same of fp32 rows, as lema_fp8_matmul_f32; the residual and out are fp32. */
+int lema_fp8_linear_f32(const void* x, int64_t ldx, const void* w, const void* sw, const void* w2,
+                        const void* sw2, const void* residual, int64_t M, int64_t N, int64_t K, void* out,
+                        void* stream);
 
 /* A token of each row of logits (laid out as in lema_token_logprobs, V at most 2^20) from u[r] in [0, 1)
  * (clamped to it; NaN as 0). With w_i = e^((z_i - max) / T) and the tokens in the order of their logits,

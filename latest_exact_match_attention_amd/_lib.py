@@ -104,6 +104,9 @@ PROTOTYPES = {
     "lema_fp8_matmul": ([_p, _p, _i64, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _p, _p, _i64, _p],
                         ctypes.c_int),
     "lema_fp8_linear": ([_p, _i32, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p], ctypes.c_int),
+    "lema_fp8_matmul_f32_workspace_bytes": ([_i64, _i64, _i64, _i32], ctypes.c_int64),
+    "lema_fp8_matmul_f32": ([_p, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _p], ctypes.c_int),
+    "lema_fp8_linear_f32": ([_p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p], ctypes.c_int),
     "lema_sample": ([_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _f32, _p, _i64, _p, _f32, _p, _f32, _p, _p,
                      _p], ctypes.c_int),
     "lema_store_exchange_view": ([_p, _i64, _i64, _p, _p, _i32, _p, _i64, _i64, _i64, _i64, _i64, _p,

@@ -7,7 +7,9 @@
 // value is rounded once, to e4m3, wherever it is quantized. The instruction aligns the products of 8
 // consecutive k to the largest of them and cuts off what lies 2^-13 below it, then adds in fp32: on
 // random blocks results are off by 1.4e-5 of the products' norm. That is far below a 16-bit
-// result's rounding, and the reason why there are no 32-bit ones.
+// result's rounding. 32-bit results (of 32-bit activations) are formed without it: a value with its scale is
+// a bf16 number (below 2^128; steps of 2^-133 below 2^-126), so both operands are widened in registers and
+// multiplied by the bf16 instruction, at a quarter of the scaled one's rate.
 //
 // Rows are held in whole blocks, zeros behind the last column.
 #include "tile_gemm.h"
@@ -25,8 +27,6 @@ __device__ __forceinline__ int scale_byte(float amax) {
   const int byte = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0);
   return max(byte, 1);
 }
-
-__device__ __forceinline__ float scale_of(int byte) { return __uint_as_float(static_cast<uint32_t>(byte) << 23); }
 
 typedef short s16x2_t __attribute__((ext_vector_type(2)));
 
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs g, uint32_
   for (int i = 0; i < kBlocks; ++i)
     if (b + i < g.blocks) {
       const int scale = scale_byte(most_of_16(v[i].amax()));
-      *reinterpret_cast<u32x2*>(to + (b + i) * 128) = v[i].fp8(scale_of(scale));
+      *reinterpret_cast<u32x2*>(to + (b + i) * 128) = v[i].fp8(power_of(scale));
       byte = lane == i ? scale : byte;
     }
   if (lane < kBlocks && b + lane < g.blocks) g.scales[(b + lane) * g.lds + row] = static_cast<uint8_t>(byte);
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(QuantArgs g) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t row = row0 + r + 16 * i;
-    if (row < g.rows) *reinterpret_cast<u32x2*>(g.values + row * g.blocks * 128 + k) = v[i].fp8(scale_of(byte));
+    if (row < g.rows) *reinterpret_cast<u32x2*>(g.values + row * g.blocks * 128 + k) = v[i].fp8(power_of(byte));
   }
   if (threadIdx.x == 0) g.scales[nb * g.lds + b] = static_cast<uint8_t>(byte);
 }
@@ -254,7 +254,17 @@ __global__ __launch_bounds__(64 * W) void fp8_small_kernel(SmallArgs g) {
         i32x8_t v;
       } xf;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) xf.h[i] = q[i].fp8(scale_of(sa));
+      for (int i = 0; i < 4; ++i) xf.h[i] = q[i].fp8(power_of(sa));
+      if constexpr (sizeof(T) == 4) {  // as bf16 (see multiply in tile_gemm.h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const Frag<Bf16> xw = widen(xf.v, i, power_of(sa));
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+            acc[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(wf[c].v, i, power_of(sb[c])).v, xw.v, acc[c][t], 0, 0, 0);
+        }
+        continue;
+      }
 #pragma unroll
       for (int c = 0; c < CT; ++c)
         acc[c][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[c].v, xf.v, acc[c][t], 0, 0, 0, sb[c], 0, sa);
@@ -296,18 +306,28 @@ using Few = Tile<Fp8, O, 64, 128, 4, false, false, kForm>;
 
 const Shape kShapes[] = {{256, 256, 1, 2.32f, 8.9f}, {128, 128, 2, 2.21f, 2.9f}, {64, 128, 2, 1.56f, 3.3f}};
 const Shape kGateShapes[] = {{256, 128, 1, 1.56f, 1.7f}, {128, 64, 2, 1.14f, 1.2f}, {64, 64, 2, 1.08f, 1.0f}};
+// 32-bit results, in Middle and Few (in Large a wave has no registers for what it widens). Fitted to 72 products of
+// 33 to 4096 rows, of which the choice takes 0.2 % longer than the best one on average, 4 % at most.
+// [65536, 6144] x 1536 takes 1182 us (1.05 PFLOP/s; into 16 bits 539), 777 x 1000 into 1234 16 us.
+const Shape kWideShapes[] = {{128, 128, 2, 2.89f, 11.4f}, {64, 128, 2, 2.29f, 7.9f}};
+const Shape kWideGateShapes[] = {{128, 64, 2, 3.59f, 12.3f}, {64, 64, 2, 2.04f, 14.5f}};
 
 int64_t blocks_in(int64_t n) { return (n + 127) / 128; }
 
-Plan plan_of(int64_t M, int64_t N, int64_t K, bool gate) {
-  return make_plan(gate ? kGateShapes : kShapes, 3, M, N, 1, gate ? 2 : 1, blocks_in(K));
+Plan plan_of(int64_t M, int64_t N, int64_t K, bool gate, bool wide) {
+  const Shape* shapes = wide ? gate ? kWideGateShapes : kWideShapes : gate ? kGateShapes : kShapes;
+  return make_plan(shapes, wide ? 2 : 3, M, N, 1, gate ? 2 : 1, blocks_in(K));
 }
 
-int check_product(int64_t M, int64_t N, int64_t K, int32_t dtype) {
-  LEMA_REQUIRE(dtype == LEMA_BF16 || dtype == LEMA_F16, "8-bit products have 16-bit results, not type %d", dtype);
+int check_product(int64_t M, int64_t N, int64_t K) {
   LEMA_REQUIRE(M >= 0 && M < (int64_t(1) << 30), "bad number of rows %lld", (long long)M);
   LEMA_REQUIRE(N > 0 && K > 0 && N <= (1 << 20) && K <= (1 << 20), "widths %lld and %lld must lie in [1, 2^20]",
                (long long)N, (long long)K);
+  return LEMA_OK;
+}
+
+int check_16(int32_t dtype) {
+  LEMA_REQUIRE(dtype == LEMA_BF16 || dtype == LEMA_F16, "results of 16 bits, not of type %d", dtype);
   return LEMA_OK;
 }
 
@@ -348,6 +368,12 @@ int product(Args& a, const Plan& p, int32_t dtype, hipStream_t st) {
            : p.shape == 1 ? launch_tiles<Middle<T, kForm>>(a, p, per_cu, st)
                           : launch_tiles<Few<T, kForm>>(a, p, per_cu, st);
   });
+}
+
+template <Form kForm>
+int wide_product(Args& a, const Plan& p, hipStream_t st) {
+  const int per_cu = (kForm == kGated ? kWideGateShapes : kWideShapes)[p.shape].per_cu;
+  return p.shape == 0 ? launch_tiles<Middle<float, kForm>>(a, p, per_cu, st) : launch_tiles<Few<float, kForm>>(a, p, per_cu, st);
 }
 
 constexpr int kSmallRows = 32;
@@ -392,16 +418,11 @@ extern "C" int lema_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int
   return dtype == LEMA_F32 ? go(0.f) : dtype == LEMA_F16 ? go(_Float16{}) : go(Bf16{});
 }
 
-extern "C" int64_t lema_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t gated) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return plan_of(M, N, K, gated != 0).part_bytes;
-}
-
-extern "C" int lema_fp8_matmul(const void* a, const void* sa, int64_t lds, const void* w, const void* sw,
-                               const void* w2, const void* sw2, int32_t dtype, int64_t M, int64_t N, int64_t K,
-                               void* out, void* ws, int64_t ws_bytes, void* stream) {
-  clear_error();
-  if (const int rc = check_product(M, N, K, dtype)) return rc;
+// A product of quantized operands, into 16 bits or (wide) 32.
+static int quantized_product(const void* a, const void* sa, int64_t lds, const void* w, const void* sw, const void* w2,
+                             const void* sw2, int32_t dtype, bool wide, int64_t M, int64_t N, int64_t K, void* out,
+                             void* ws, int64_t ws_bytes, void* stream) {
+  if (const int rc = check_product(M, N, K)) return rc;
   const bool gate = w2 != nullptr;
   LEMA_REQUIRE(!gate || N % 8 == 0, "a gated product's width %lld must be a multiple of 8", (long long)N);
   LEMA_REQUIRE(lds >= M && lds % 4 == 0, "the scales' stride %lld must be a multiple of 4, at least the rows",
@@ -410,7 +431,7 @@ extern "C" int lema_fp8_matmul(const void* a, const void* sa, int64_t lds, const
   LEMA_REQUIRE(a && sa && w && sw && out && (!gate || sw2), "bad pointer");
   LEMA_REQUIRE(aligned(a, 16) && aligned(w, 16) && aligned(w2, 16) && aligned(out, 16) && aligned(sa, 4),
                "the operands must lie at multiples of 16 bytes, the scales of 4");
-  const Plan p = plan_of(M, N, K, gate);
+  const Plan p = plan_of(M, N, K, gate, wide);
   LEMA_REQUIRE(p.part_bytes == 0 || (ws && aligned(ws, 16) && ws_bytes >= p.part_bytes),
                "the workspace must hold %lld bytes", (long long)p.part_bytes);
   const int64_t blocks = blocks_in(K);
@@ -432,19 +453,45 @@ extern "C" int lema_fp8_matmul(const void* a, const void* sa, int64_t lds, const
   g.nk = static_cast<int32_t>(blocks);
   g.segs = 1;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (wide) return gate ? wide_product<kGated>(g, p, st) : wide_product<kPlain>(g, p, st);
   return gate ? product<kGated>(g, p, dtype, st) : product<kPlain>(g, p, dtype, st);
 }
 
-extern "C" int lema_fp8_linear(const void* x, int32_t dtype, int64_t ldx, const void* w, const void* sw,
-                               const void* w2, const void* sw2, const void* residual, int64_t M, int64_t N,
-                               int64_t K, void* out, void* stream) {
+extern "C" int64_t lema_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t gated) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return plan_of(M, N, K, gated != 0, false).part_bytes;
+}
+
+extern "C" int lema_fp8_matmul(const void* a, const void* sa, int64_t lds, const void* w, const void* sw,
+                               const void* w2, const void* sw2, int32_t dtype, int64_t M, int64_t N, int64_t K,
+                               void* out, void* ws, int64_t ws_bytes, void* stream) {
   clear_error();
-  if (const int rc = check_product(M, N, K, dtype)) return rc;
+  if (const int rc = check_16(dtype)) return rc;
+  return quantized_product(a, sa, lds, w, sw, w2, sw2, dtype, false, M, N, K, out, ws, ws_bytes, stream);
+}
+
+extern "C" int64_t lema_fp8_matmul_f32_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t gated) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return plan_of(M, N, K, gated != 0, true).part_bytes;
+}
+
+extern "C" int lema_fp8_matmul_f32(const void* a, const void* sa, int64_t lds, const void* w, const void* sw,
+                                   const void* w2, const void* sw2, int64_t M, int64_t N, int64_t K, void* out,
+                                   void* ws, int64_t ws_bytes, void* stream) {
+  clear_error();
+  return quantized_product(a, sa, lds, w, sw, w2, sw2, LEMA_F32, true, M, N, K, out, ws, ws_bytes, stream);
+}
+
+// A product of at most 32 rows that the launch quantizes, into the rows' type.
+static int small_product(const void* x, int32_t dtype, int64_t ldx, const void* w, const void* sw, const void* w2,
+                         const void* sw2, const void* residual, int64_t M, int64_t N, int64_t K, void* out, void* stream) {
+  if (const int rc = check_product(M, N, K)) return rc;
   LEMA_REQUIRE(M <= kSmallRows, "%lld rows: this launch takes at most %d", (long long)M, kSmallRows);
   LEMA_REQUIRE(ldx >= K, "row stride %lld is below %lld", (long long)ldx, (long long)K);
   if (M == 0) return LEMA_OK;
   LEMA_REQUIRE(x && w && sw && out && (!w2 || sw2), "bad pointer");
-  LEMA_REQUIRE(aligned(x, 2) && aligned(w, 16) && aligned(w2, 16) && aligned(out, 2) && aligned(residual, 2),
+  const int size = dtype_size(dtype);
+  LEMA_REQUIRE(aligned(x, size) && aligned(w, 16) && aligned(w2, 16) && aligned(out, size) && aligned(residual, size),
                "the weights must lie at multiples of 16 bytes");
   SmallArgs g{x,
               {static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(w2)},
@@ -457,8 +504,24 @@ extern "C" int lema_fp8_linear(const void* x, int32_t dtype, int64_t ldx, const 
               static_cast<int32_t>(K),
               static_cast<int32_t>(blocks_in(K))};
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == LEMA_F32) return w2 ? launch_small<float, true>(g, st) : launch_small<float, false>(g, st);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     return w2 ? launch_small<T, true>(g, st) : launch_small<T, false>(g, st);
   });
+}
+
+extern "C" int lema_fp8_linear(const void* x, int32_t dtype, int64_t ldx, const void* w, const void* sw,
+                               const void* w2, const void* sw2, const void* residual, int64_t M, int64_t N,
+                               int64_t K, void* out, void* stream) {
+  clear_error();
+  if (const int rc = check_16(dtype)) return rc;
+  return small_product(x, dtype, ldx, w, sw, w2, sw2, residual, M, N, K, out, stream);
+}
+
+extern "C" int lema_fp8_linear_f32(const void* x, int64_t ldx, const void* w, const void* sw, const void* w2,
+                                   const void* sw2, const void* residual, int64_t M, int64_t N, int64_t K, void* out,
+                                   void* stream) {
+  clear_error();
+  return small_product(x, LEMA_F32, ldx, w, sw, w2, sw2, residual, M, N, K, out, stream);
 }

@@ -11,9 +11,11 @@ A block is 128 columns of one row (activations) or of 128 rows (weights). Its sc
 of two 2^e, e >= -126, that brings its largest finite value to at most 448, so that x / 2^e is exact and
 a value is rounded once, to the nearest e4m3, halves to even; the scales are held as e8m0. A block of
 zeros has the scale 1. Infinities and NaN become NaN, and reach their row (or weight's column) of the
-result. Products are summed up in fp32, but for those of 8 consecutive columns, which the matrix
-instruction aligns to the largest of them and cuts off 2^-13 below it (1.4e-5 of the products' norm on
-random blocks); results are bfloat16 or float16. Nothing here has a gradient.
+result. Products are summed up in fp32. Into bfloat16 and float16 those of 8 consecutive columns go by an
+instruction that aligns them to the largest of them and cuts off what lies 2^-13 below it (1.4e-5 of the
+products' norm on random blocks). Into float32 every product is exact, at half of the speed, and the
+values are those that bfloat16 holds: infinite from 2^128 on, in steps of 2^-133 below 2^-126. Nothing
+here has a gradient.
 """
 from __future__ import annotations
 
@@ -121,8 +123,8 @@ def _weight(name: str, w: Fp8, K: int, like: torch.Tensor):
 
 
 def _result_type(dtype):
-    if dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"8-bit products take and give bfloat16 or float16, not {dtype}")
+    if dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"8-bit products take and give float32, bfloat16 or float16, not {dtype}")
 
 
 def _product(values, scales, lds, M, K, w, w2, dtype, shape):
@@ -131,18 +133,21 @@ def _product(values, scales, lds, M, K, w, w2, dtype, shape):
     N = v.shape[0]
     out = values.new_empty(shape + (N,), dtype=dtype)
     L = _lib.lib()
-    n = L.lema_fp8_matmul_workspace_bytes(M, N, K, w2 is not None)
+    wide = dtype is torch.float32
+    size = L.lema_fp8_matmul_f32_workspace_bytes if wide else L.lema_fp8_matmul_workspace_bytes
+    n = size(M, N, K, w2 is not None)
     ws = values.new_empty(n, dtype=torch.uint8) if n else None
+    operands = (values.data_ptr(), scales.data_ptr(), lds, v.data_ptr(), s.data_ptr(), _ptr(v2), _ptr(s2))
+    rest = (M, N, K, out.data_ptr(), _ptr(ws), n, _lib.stream_of(values))
     with _lib.device_of(values):
-        _lib.check(L.lema_fp8_matmul(
-            values.data_ptr(), scales.data_ptr(), lds, v.data_ptr(), s.data_ptr(), _ptr(v2), _ptr(s2),
-            _lib.DTYPE_CODE[dtype], M, N, K, out.data_ptr(), _ptr(ws), n, _lib.stream_of(values)))
+        _lib.check(L.lema_fp8_matmul_f32(*operands, *rest) if wide else
+                   L.lema_fp8_matmul(*operands, _lib.DTYPE_CODE[dtype], *rest))
     return out
 
 
 def matmul(a: Fp8, w: Fp8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a . w^T: a [..., K] with a scale for each row's blocks, w [N, K] with one for each 128 x 128;
-    [..., N] in bfloat16 or float16."""
+    [..., N] in float32, bfloat16 or float16."""
     _result_type(dtype)
     K, lead = a.columns, a.values.shape[:-1]
     _lib.require_device(a.values, a.scales)
@@ -185,10 +190,11 @@ def _linear(x, w, w2, residual):
         return y if residual is None else y.add_(residual)
     out = x.new_empty(lead + (N,))
     (v, s), (v2, s2) = w, w2 or (None, None)
+    L = _lib.lib()
+    rest = (K, v.data_ptr(), s.data_ptr(), _ptr(v2), _ptr(s2), _ptr(residual), M, N, K, out.data_ptr(), _lib.stream_of(x))
     with _lib.device_of(x):
-        _lib.check(_lib.lib().lema_fp8_linear(
-            x.data_ptr(), _lib.DTYPE_CODE[x.dtype], K, v.data_ptr(), s.data_ptr(), _ptr(v2), _ptr(s2),
-            _ptr(residual), M, N, K, out.data_ptr(), _lib.stream_of(x)))
+        _lib.check(L.lema_fp8_linear_f32(x.data_ptr(), *rest) if x.dtype is torch.float32 else
+                   L.lema_fp8_linear(x.data_ptr(), _lib.DTYPE_CODE[x.dtype], *rest))
     return out
 
 
@@ -201,9 +207,9 @@ def _input(x, *others):
 
 
 def linear(x: torch.Tensor, w: Fp8, residual: torch.Tensor | None = None) -> torch.Tensor:
-    """x . w^T (+ residual), x [..., K] in bfloat16 or float16, quantized for each row's blocks: one
-    launch up to 32 rows, a quantizing pass and a product beyond. The product is rounded to x's type
-    before the residual [..., N] is added."""
+    """x . w^T (+ residual) in x's type, x [..., K] in float32, bfloat16 or float16, quantized for each
+    row's blocks: one launch up to 32 rows, a quantizing pass and a product beyond. The product is rounded
+    to x's type before the residual [..., N] is added."""
     _input(x, residual)
     w = _weight("w", w, x.shape[-1], x)
     if residual is not None:

@@ -40,3 +40,19 @@ def hip():
 def dev(hip):
     import torch
     return torch.device("cuda", 0)
+
+
+# Tests that hold what was mended after them. They stay as they were, run, and must fail: a test
+# of what holds now stands beside each.
+OVERTAKEN = {
+    "test_gpu_fp8.py::test_refusals":
+        "holds that 8-bit products refuse 32-bit activations, without which a model that nobody cast could be "
+        "held in 8 bits but not run; test_gpu_fp8_f32.py has its other refusals",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        for name, reason in OVERTAKEN.items():
+            if item.nodeid.endswith(name):
+                item.add_marker(pytest.mark.xfail(reason=reason, strict=True))
