@@ -5,7 +5,7 @@ Three kinds:
   gated   the feed-forward block's input: silu(x . Wg^T) * (x . Wu^T); with `grad` the gradients of
           x and both weights
   fp8     x . W^T in 8-bit floating point (e4m3) with power-of-two scales: one for each 128 columns
-          of a row of x, one for each 128 x 128 block of W; x and the result in 16 bits
+          of a row of x, one for each 128 x 128 block of W; x comes in 16 or 32 bits
   sample  a token of each row of logits from a given random number, after temperature, top-k, top-p
           and min-p; and its log-probability at that temperature
 
@@ -77,7 +77,7 @@ def draw(rng):
         N = min(N, (1 << 27) // K)
         K, N = (K, N) if rng.random() < 0.3 else (_eights(K), _eights(N))
         rows = max(1, min(_log(rng, 1, 65536), 65536 * 6144 * 1536 // (K * N)))
-        return dict(kind=kind, rows=rows, K=K, N=N, dtype=rng.choice(["bf16", "bf16", "f16"]))
+        return dict(kind=kind, rows=rows, K=K, N=N, dtype=rng.choice(["bf16", "bf16", "f16", "f32"]))
     vocab = _log(rng, 1000, 131072)
     vocab = vocab if rng.random() < 0.3 else _eights(vocab)
     dtype = rng.choice(["bf16", "bf16", "f16", "f32"])
