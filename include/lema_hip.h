@@ -458,6 +458,11 @@ int lema_skinny_swiglu_bf16(const void* x, int64_t ldx, const void* wg, const vo
                             int64_t ldw, int64_t M, int64_t N, int64_t K, void* out,
                             void* stream);
 
+/* The same from the fp32 sums, out[M, N] = bf16(silu(x . wg^T) * (x . wu^T)): rounded as lema_gated_linear
+ * rounds it. */
+int lema_skinny_gated_bf16(const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw,
+                           int64_t M, int64_t N, int64_t K, void* out, void* stream);
+
 /* The MLP input of a decode step and its gate and up products in one launch
  * (code/lema/model.py:229-232, 85-94): s = x + d (each sum rounded to bf16; d NULL: s = x),
  * h = bf16(s * rsqrt(mean(s^2) + eps) * nw) rounded exactly as lema_rmsnorm_bf16 rounds it,
@@ -467,6 +472,11 @@ int lema_skinny_swiglu_bf16(const void* x, int64_t ldx, const void* wg, const vo
 int lema_skinny_norm_swiglu_bf16(const void* x, const void* d, const void* nw, float eps,
                                  void* x_out, const void* wg, const void* wu, int64_t ldw,
                                  int64_t M, int64_t N, int64_t K, void* out, void* stream);
+
+/* The same with lema_skinny_gated_bf16 of h. */
+int lema_skinny_norm_gated_bf16(const void* x, const void* d, const void* nw, float eps, void* x_out,
+                                const void* wg, const void* wu, int64_t ldw, int64_t M, int64_t N,
+                                int64_t K, void* out, void* stream);
 
 /* The attention input of a decode step and its q, k and v projections in one launch
  * (code/lema/model.py:224-227, 168-175): h = bf16(x * rsqrt(mean(x^2) + eps) * nw) rounded

@@ -14,9 +14,11 @@
 //           head's code is (bf16(z_j) >= 0), the sign of the value the unfused path would have
 //           stored -- the projection's output never goes to HBM. A block covers 16 columns and
 //           writes the bytes of each code its columns hold (d a multiple of 8), or whole heads;
-//   swiglu  silu(x . gate^T) * (x . up^T) with the same bf16 roundings as SwiGLU.forward's
-//           ops (code/lema/model.py:85-94): the block computes 16 columns of both.
-// A swiglu launch can also take the MLP's pre-norm (Block.forward's norm2 with the attention's
+//   gated   silu(x . gate^T) * (x . up^T) (code/lema/model.py:85-94) from the fp32 sums, rounded once, as
+//           the gated product of more rows (gated.hip) rounds it: the block computes 16 columns of both;
+//   swiglu  the same with both products and the silu rounded to bf16 on the way, as swiglu of two
+//           linear products rounds them, which widths that are no multiple of 8 take elsewhere.
+// A gated or swiglu launch can also take the MLP's pre-norm (Block.forward's norm2 with the attention's
 // residual add, code/lema/model.py:229-232): every block then forms the normalised rows
 // itself, with the stand-alone norm kernel's arithmetic (norm_row.h), into LDS and multiplies
 // those; block 0 also writes x + d, the MLP's residual. That saves the norm's launch. A q/k/v
@@ -45,12 +47,12 @@ constexpr int kSkNormMaxK = 8 * kSkStepK;  // longest rows of a fused pre-norm, 
 // One weight segment of a launch: its blocks cover N output columns of x . w^T with one
 // epilogue. A launch holds up to three segments sharing x (the q, k and v projections of a
 // layer in one launch).
-enum SkMode : int32_t { kSkPlain = 0, kSkPack = 1, kSkSwiglu = 2 };
+enum SkMode : int32_t { kSkPlain = 0, kSkPack = 1, kSkSwiglu = 2, kSkGated = 3 };
 
 struct SkSegment {
   const uint16_t* w;   // [N, K]
-  const uint16_t* w2;  // swiglu: the up projection [N, K] (w is the gate)
-  void* out;           // plain / swiglu: bf16 [M, ldy]; pack: codes
+  const uint16_t* w2;  // gated, swiglu: the up projection [N, K] (w is the gate)
+  void* out;           // pack: codes; else bf16 [M, ldy]
   const uint16_t* res; // plain: optional bf16 [M, ldy] residual, out = bf16(res + bf16(sum))
   int64_t ldy;
   int32_t N, mode, code_bytes;
@@ -93,7 +95,7 @@ struct SkDevice {
   uint32_t flags;        // mode | segments << 2 | code bytes << 4 | columns per block << 8 | M << 16
                          // | the strides' next 5 bits << 22 (x) and << 27 (weights)
   int32_t blocks;        // of the first segment, and of the second
-  const uint16_t* w1;    // the second segment's, or swiglu's up
+  const uint16_t* w1;    // the second segment's, or a gate's up
   const uint16_t* w2;    // the third segment's: plain, Nv columns
   void* out1;
   void* out2;
@@ -172,7 +174,7 @@ __global__ __launch_bounds__(kSkThreads, MT * CT <= 2 && (kNorm != 0 ? U <= 6 : 
     N = s2 ? a.Nv : N;
     bid -= s2 ? 2 * a.blocks : s1 ? a.blocks : 0;
   }
-  const bool glu = mode == kSkSwiglu;
+  const bool glu = mode >= kSkSwiglu;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
   const int64_t ldx = (static_cast<int64_t>((a.flags >> 22) & 31) << 32 | a.ldx8) * 8;
   const int64_t ldw = (static_cast<int64_t>(a.flags >> 27) << 32 | a.ldw8) * 8;
@@ -379,16 +381,18 @@ __global__ __launch_bounds__(kSkThreads, MT * CT <= 2 && (kNorm != 0 ? U <= 6 : 
     return;
   }
   if constexpr (CT == 2) {
-    if (glu) {  // out = silu(gate) * up, the silu rounded to bf16 first; up is 16 lanes on
+    if (glu) {  // out = silu(gate) * up; up is 16 lanes on
       uint16_t* y = static_cast<uint16_t*>(dst);
+      const bool once = mode == kSkGated;
+      auto rounded = [&](float f) { return once ? f : bf16_bits_to_f32(f32_to_bf16_bits(f)); };
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int e = threadIdx.x + i * kSkThreads;
         const int row = e / kCols, c = e % kCols;
-        const float u = bf16_bits_to_f32(f32_to_bf16_bits(__shfl(sums[i], l | 16)));
+        const float u = rounded(__shfl(sums[i], l | 16));
         if (c >= 16 || row >= M || n0 + c >= N) continue;
-        const float g = bf16_bits_to_f32(f32_to_bf16_bits(sums[i]));
-        const float sl = bf16_bits_to_f32(f32_to_bf16_bits(g / (1.0f + expf(-g))));
+        const float g = rounded(sums[i]);
+        const float sl = rounded(g / (1.0f + expf(-g)));
         y[static_cast<int64_t>(row) * a.ldy + n0 + c] = static_cast<uint16_t>(f32_to_bf16_bits(sl * u));
       }
       return;
@@ -451,7 +455,7 @@ int launch_skinny(SkinnyArgs& a, hipStream_t st) {
   for (int j = 0; j < a.nseg; ++j) all_plain = all_plain && a.seg[j].mode == kSkPlain;
   const SkSegment& s0 = a.seg[0];
   const bool narrow = CT == 1 && all_plain && s0.N <= kNarrowMaxN;
-  const int cols = s0.mode == kSkSwiglu ? 16 : narrow ? kNarrowCols : 16 * CT;
+  const int cols = s0.mode >= kSkSwiglu ? 16 : narrow ? kNarrowCols : 16 * CT;
   int blocks = 0;
   for (int i = 0; i < a.nseg; ++i) blocks += (a.seg[i].N + cols - 1) / cols;
   SkDevice g{};
@@ -724,10 +728,8 @@ extern "C" int lema_skinny_norm_qkv_bf16(const void* x, const void* nw, float ep
   return launch_ct(a, ct, static_cast<hipStream_t>(stream));
 }
 
-extern "C" int lema_skinny_swiglu_bf16(const void* x, int64_t ldx, const void* wg, const void* wu,
-                                       int64_t ldw, int64_t M, int64_t N, int64_t K, void* out,
-                                       void* stream) {
-  clear_error();
+static int gate_up(SkMode mode, const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw, int64_t M,
+                   int64_t N, int64_t K, void* out, void* stream) {
   if (int rc = check_skinny(x, ldx, ldw, M, K)) return rc;
   if (int rc = check_weight(wg, N)) return rc;
   if (int rc = check_weight(wu, N)) return rc;
@@ -740,15 +742,27 @@ extern "C" int lema_skinny_swiglu_bf16(const void* x, int64_t ldx, const void* w
   a.K = static_cast<int32_t>(K);
   a.nseg = 1;
   a.seg[0] = SkSegment{static_cast<const uint16_t*>(wg), static_cast<const uint16_t*>(wu), out,
-                       nullptr, N, static_cast<int32_t>(N), kSkSwiglu, 0};
+                       nullptr, N, static_cast<int32_t>(N), mode, 0};
   return launch_ct(a, 2, static_cast<hipStream_t>(stream));
 }
 
-extern "C" int lema_skinny_norm_swiglu_bf16(const void* x, const void* d, const void* nw,
-                                            float eps, void* x_out, const void* wg,
-                                            const void* wu, int64_t ldw, int64_t M, int64_t N,
-                                            int64_t K, void* out, void* stream) {
+extern "C" int lema_skinny_gated_bf16(const void* x, int64_t ldx, const void* wg, const void* wu,
+                                      int64_t ldw, int64_t M, int64_t N, int64_t K, void* out,
+                                      void* stream) {
   clear_error();
+  return gate_up(kSkGated, x, ldx, wg, wu, ldw, M, N, K, out, stream);
+}
+
+extern "C" int lema_skinny_swiglu_bf16(const void* x, int64_t ldx, const void* wg, const void* wu,
+                                       int64_t ldw, int64_t M, int64_t N, int64_t K, void* out,
+                                       void* stream) {
+  clear_error();
+  return gate_up(kSkSwiglu, x, ldx, wg, wu, ldw, M, N, K, out, stream);
+}
+
+static int norm_gate_up(SkMode mode, const void* x, const void* d, const void* nw, float eps, void* x_out,
+                        const void* wg, const void* wu, int64_t ldw, int64_t M, int64_t N, int64_t K, void* out,
+                        void* stream) {
   if (int rc = check_skinny(x, K, ldw, M, K)) return rc;
   if (int rc = check_weight(wg, N)) return rc;
   if (int rc = check_weight(wu, N)) return rc;
@@ -771,10 +785,24 @@ extern "C" int lema_skinny_norm_swiglu_bf16(const void* x, const void* d, const 
   a.K = static_cast<int32_t>(K);
   a.nseg = 1;
   a.seg[0] = SkSegment{static_cast<const uint16_t*>(wg), static_cast<const uint16_t*>(wu), out,
-                       nullptr, N, static_cast<int32_t>(N), kSkSwiglu, 0};
+                       nullptr, N, static_cast<int32_t>(N), mode, 0};
   a.nd = static_cast<const uint16_t*>(d);
   a.nw = static_cast<const uint16_t*>(nw);
   a.ns = static_cast<uint16_t*>(x_out);
   a.eps = eps;
   return launch_ct(a, 2, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int lema_skinny_norm_gated_bf16(const void* x, const void* d, const void* nw, float eps, void* x_out,
+                                           const void* wg, const void* wu, int64_t ldw, int64_t M, int64_t N,
+                                           int64_t K, void* out, void* stream) {
+  clear_error();
+  return norm_gate_up(kSkGated, x, d, nw, eps, x_out, wg, wu, ldw, M, N, K, out, stream);
+}
+
+extern "C" int lema_skinny_norm_swiglu_bf16(const void* x, const void* d, const void* nw, float eps, void* x_out,
+                                            const void* wg, const void* wu, int64_t ldw, int64_t M, int64_t N,
+                                            int64_t K, void* out, void* stream) {
+  clear_error();
+  return norm_gate_up(kSkSwiglu, x, d, nw, eps, x_out, wg, wu, ldw, M, N, K, out, stream);
 }

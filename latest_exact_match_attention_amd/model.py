@@ -649,9 +649,10 @@ class SwiGLU(nn.Module):
 
     def forward(self, x, residual=None):
         """down(silu(gate(x)) * up(x)), plus `residual` when given (Block's x + mlp(h)). On
-        decode shapes the gate, up and product are one launch and the down projection adds
-        the residual in its epilogue; longer inputs take gated_linear, and in bf16 without
-        autograd the down GEMM accumulates into `residual` itself, which is then returned."""
+        decode shapes the gate, up and product are one launch, rounded as gated_linear rounds
+        them, and the down projection adds the residual in its epilogue; longer inputs take
+        gated_linear, and in bf16 without autograd the down GEMM accumulates into `residual`
+        itself, which is then returned."""
         if self._fp8():
             a = (fp8.gated_linear(x, self.gate.weight, self.up.weight)
                  if self.gate.out_features % 8 == 0 else swiglu(self.gate(x), self.up(x)))
@@ -662,7 +663,9 @@ class SwiGLU(nn.Module):
             K, N = x.shape[-1], g.shape[0]
             M = x.numel() // K
             a = x.new_empty(x.shape[:-1] + (N,))
-            _lib.check(_lib.lib().lema_skinny_swiglu_bf16(
+            L = _lib.lib()
+            # (widths that gated_linear does not take keep the roundings that they have there)
+            _lib.check((L.lema_skinny_gated_bf16 if N % 8 == 0 else L.lema_skinny_swiglu_bf16)(
                 x.data_ptr(), K, g.data_ptr(), u.data_ptr(), K, M, N, K, a.data_ptr(),
                 _lib.stream_of(x)))
             if residual is not None and _skinny(a, dn) and residual.is_contiguous() \
@@ -674,10 +677,7 @@ class SwiGLU(nn.Module):
                     dn.shape[0], M, dn.shape[0], N, _lib.stream_of(x)))
                 return y
         else:
-            # decode shapes keep the roundings of their one launch where they take it apart for a
-            # gradient
-            a = (swiglu(linear(x, self.gate), linear(x, self.up)) if _skinny(x, g)
-                 else gated_linear(x, self.gate, self.up))
+            a = gated_linear(x, self.gate, self.up)
             if residual is not None and not _skinny(a, dn) and a.is_cuda and \
                     a.dtype == residual.dtype == dn.dtype == torch.bfloat16 and \
                     residual.is_contiguous() and not torch.is_grad_enabled():
@@ -713,7 +713,7 @@ class SwiGLU(nn.Module):
         xo = torch.empty_like(x)
         a = x.new_empty(x.shape[:-1] + (N,))
         eps = norm.eps if norm.eps is not None else torch.finfo(x.dtype).eps
-        _lib.check(_lib.lib().lema_skinny_norm_swiglu_bf16(
+        _lib.check(_lib.lib().lema_skinny_norm_gated_bf16(
             x.data_ptr(), d.data_ptr(), norm.weight.data_ptr(), float(eps), xo.data_ptr(),
             g.data_ptr(), u.data_ptr(), K, M, N, K, a.data_ptr(), _lib.stream_of(x)))
         y = torch.empty_like(xo)
@@ -887,7 +887,8 @@ class Transformer(nn.Module):
             forward(next, cache=c)                    extending c
 
         With a cache, queries match keys from before this call too, so a sequence can be fed
-        in pieces; any chunking gives the one-shot result. In bf16 on the GPU nothing of a call
+        in pieces: every piece's numbers are rounded alike, though a 16-bit sum's last bit can
+        depend on how many rows a call has (another order of its terms in fp32). In bf16 on the GPU nothing of a call
         with a cache has a gradient, its logits neither. Tokens must lie in [0, vocab_size); on the
         GPU they are not checked.
         """
