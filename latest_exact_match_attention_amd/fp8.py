@@ -253,6 +253,14 @@ class Fp8Linear(nn.Module):
             raise ValueError("an 8-bit linear layer has no bias")
         return cls(quantize(lin.weight.detach(), BLOCK))
 
+    @classmethod
+    def blank(cls, out_features: int, in_features: int, device=None) -> "Fp8Linear":
+        """A weight of zeros, to load a state_dict into."""
+        kb = _blocks(in_features)
+        values = torch.zeros(out_features, kb * BLOCK, dtype=torch.uint8, device=device)
+        scales = torch.full((_blocks(out_features), kb), 127, dtype=torch.uint8, device=device)
+        return cls(Fp8(values.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu), in_features))
+
     @property
     def weight(self) -> Fp8:
         return Fp8(self.values.view(torch.float8_e4m3fn), self.scales.view(torch.float8_e8m0fnu), self.in_features)
@@ -268,7 +276,7 @@ def quantize_feed_forward(model: nn.Module, head: bool = False) -> nn.Module:
     """Holds the feed-forward weights of a Transformer's blocks (and with `head` the head's) in 8 bits, in
     place, for serving; returns the model. The query and key projections keep their type: their
     outputs' signs are the codes that are matched exactly, and the value and output projections are
-    small beside the feed-forward ones."""
+    small beside the feed-forward ones. A model's state_dict then loads into one that was held so, too."""
     for block in model.blocks:
         for name in ("gate", "up", "down"):
             lin = getattr(block.mlp, name)

@@ -55,9 +55,9 @@ __all__ = ["ModelConfig", "SwiGLU", "Attention", "Block", "Transformer", "lm_los
 
 def _fused(*ts: torch.Tensor) -> bool:
     """Whether the kernels take the tensors as they lie: bf16 on the GPU, contiguous, from a 16-byte
-    boundary on (a slice, or a parameter in a flat buffer, may start elsewhere)."""
+    boundary on (a slice, or a parameter in a flat buffer, may start elsewhere). An 8-bit weight is none."""
     for t in ts:
-        if not (t.is_cuda and t.dtype is torch.bfloat16 and t.is_contiguous() and t.data_ptr() % 16 == 0):
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is torch.bfloat16 and t.is_contiguous() and t.data_ptr() % 16 == 0):
             return False
     return True
 
@@ -377,6 +377,8 @@ def gated_linear(x: torch.Tensor, gate: nn.Linear, up: nn.Linear) -> torch.Tenso
     Differentiable in x and both weights; for the gradient the forward keeps the result's derivatives by
     both products, in 20 bits. Widths that are multiples of 8, up to 2^20. Other widths, types and devices, modules with
     a bias, hooks or a forward of their own, and torch.autocast take linear and swiglu."""
+    if isinstance(gate, fp8.Fp8Linear) or isinstance(up, fp8.Fp8Linear):
+        return swiglu(linear(x, gate), linear(x, up))
     wg, wu = gate.weight, up.weight
     K = x.shape[-1] if x.dim() else 0
     if not (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and wg.dtype is wu.dtype is x.dtype
@@ -480,7 +482,7 @@ class _SkinnyLinear(torch.autograd.Function):
 
 def linear(x: torch.Tensor, lin: nn.Linear) -> torch.Tensor:
     """lin(x); a decode-shaped product (<= 32 rows, bf16) on the skinny MFMA kernel."""
-    if type(lin) is fp8.Fp8Linear or not _skinny(x, lin.weight):
+    if isinstance(lin, fp8.Fp8Linear) or not _skinny(x, lin.weight):
         return lin(x)
     if _lib.needs_grad(x, lin.weight):
         return _SkinnyLinear.apply(x, lin.weight)
@@ -516,9 +518,8 @@ def project_qkv(x: torch.Tensor, at, code_dtype: torch.dtype, norm: nn.RMSNorm |
     apply."""
     c = at.cfg
     wq, wk, wv = at.q_proj.weight, at.k_proj.weight, at.v_proj.weight
-    if not (_skinny(x, wq) and x.dim() == 3 and wq.shape == wk.shape and _pack_tiles(c.d_qk)
-            and wk.data_ptr() % 16 == 0 and wv.data_ptr() % 16 == 0
-            and wv.dtype == wq.dtype and wv.is_contiguous() and wk.is_contiguous()):
+    if not (_skinny(x, wq) and x.dim() == 3 and _fused(wk, wv) and wq.shape == wk.shape
+            and _pack_tiles(c.d_qk)):
         return None
     B, T, K = x.shape
     Nqk, Nv = wq.shape[0], wv.shape[0]
@@ -566,9 +567,9 @@ def project_qk_prefill(x: torch.Tensor, at, code_dtype: torch.dtype):
     where the launch does not apply (the caller then projects and packs)."""
     c = at.cfg
     wq, wk = at.q_proj.weight, at.k_proj.weight
-    if torch.is_grad_enabled() and (x.requires_grad or wq.requires_grad or wk.requires_grad):
-        return None
     if not (_fused(x, wq, wk) and x.dim() == 3 and wq.shape == wk.shape):
+        return None
+    if torch.is_grad_enabled() and (x.requires_grad or wq.requires_grad or wk.requires_grad):
         return None
     B, T, K = x.shape
     N, d = wq.shape[0], c.d_qk
@@ -654,9 +655,14 @@ class SwiGLU(nn.Module):
         gated_linear, and in bf16 without autograd the down GEMM accumulates into `residual`
         itself, which is then returned."""
         if self._fp8():
-            a = (fp8.gated_linear(x, self.gate.weight, self.up.weight)
-                 if self.gate.out_features % 8 == 0 else swiglu(self.gate(x), self.up(x)))
-            return self.down(a, residual)
+            gated = (isinstance(self.gate, fp8.Fp8Linear) and isinstance(self.up, fp8.Fp8Linear)
+                     and self.gate.out_features % 8 == 0)
+            a = (fp8.gated_linear(x, self.gate.weight, self.up.weight) if gated
+                 else gated_linear(x, self.gate, self.up))
+            if isinstance(self.down, fp8.Fp8Linear):
+                return self.down(a, residual)
+            y = linear(a, self.down)
+            return y if residual is None else residual + y
         g, u, dn = self.gate.weight, self.up.weight, self.down.weight
         if _skinny(x, g) and g.shape == u.shape and u.data_ptr() % 16 == 0 and u.is_contiguous() \
                 and not _lib.needs_grad(x, g, u, dn, residual):
@@ -691,8 +697,8 @@ class SwiGLU(nn.Module):
         return y if residual is None else residual + y
 
     def _fp8(self) -> bool:
-        """Whether the weights are held in 8 bits, all three."""
-        return type(self.gate) is type(self.up) is type(self.down) is fp8.Fp8Linear
+        """Whether one of the weights is held in 8 bits."""
+        return any(isinstance(lin, fp8.Fp8Linear) for lin in (self.gate, self.up, self.down))
 
     def forward_normed(self, x, d, norm: nn.RMSNorm):
         """x + d + self(norm(x + d)), Block.forward's MLP half, on decode shapes: the norm runs
@@ -919,8 +925,9 @@ class Transformer(nn.Module):
 
     def n_params(self, embedding: bool = True) -> int:
         n = sum(p.numel() for p in self.parameters())
+        n += sum(m.out_features * m.in_features for m in self.modules() if isinstance(m, fp8.Fp8Linear))
         if not embedding:
-            n -= self.tok_emb.weight.numel() + self.lm_head.weight.numel()
+            n -= self.tok_emb.weight.numel() + self.lm_head.out_features * self.lm_head.in_features
         return n
 
 
@@ -945,7 +952,8 @@ def load_trained(path, device="cuda") -> tuple[Transformer, ModelConfig]:
     """A finished training run, ready to evaluate (code/lema/model.py:420-436): `path` is the
     run directory (its `model.pt`) or a checkpoint file, a dict holding `config` (the
     ModelConfig fields) and `state_dict`. The model comes back in hard mode, fp32, in eval
-    mode; parameters the checkpoint holds beyond this model's are dropped.
+    mode; parameters the checkpoint holds beyond this model's are dropped. Linear layers that
+    it holds in 8 bits (`fp8.quantize_feed_forward`) come back so.
 
     The file is read with `torch.load(weights_only=True)`, which builds tensors and plain
     containers only and executes nothing from the file; a checkpoint that needs arbitrary
@@ -959,6 +967,11 @@ def load_trained(path, device="cuda") -> tuple[Transformer, ModelConfig]:
         raise ValueError(f"{path}: expected a dict with 'config' and 'state_dict'")
     cfg = ModelConfig.from_dict(dict(ck["config"]))
     model = Transformer(cfg).to(device).eval()
+    for name, mod in list(model.named_modules()):
+        if isinstance(mod, nn.Linear) and name + ".scales" in ck["state_dict"]:
+            owner, _, leaf = name.rpartition(".")
+            setattr(model.get_submodule(owner), leaf,
+                    fp8.Fp8Linear.blank(mod.out_features, mod.in_features, device))
     keep = model.state_dict().keys()
     model.load_state_dict({k: v for k, v in ck["state_dict"].items() if k in keep})
     model.set_hard(True)
