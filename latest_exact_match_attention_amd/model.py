@@ -338,6 +338,16 @@ def _gated_forward(x, wg, wu, keep):
     return y, slopes
 
 
+def _gated_grad_ops(gy, x, wg, wu):
+    """The gradients of gated_linear in torch's operations, which have gradients of their own and compose with
+    functional transforms."""
+    g, u, x2 = F.linear(x, wg).float(), F.linear(x, wu).float(), x.reshape(-1, x.shape[-1])
+    s = torch.sigmoid(g)
+    dg, du = ((gy.float() * d).to(x.dtype) for d in (u * s * (1 + g * (1 - s)), g * s))
+    gw = ((d.reshape(-1, d.shape[-1]).t() @ x2) for d in (dg, du))
+    return F.linear(dg, wg.t()) + F.linear(du, wu.t()), *gw
+
+
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu):
@@ -346,8 +356,17 @@ class _GatedLinear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @_lib.once
     def backward(ctx, gy):
+        # float16 had torch's operations before it had this kernel: what they take is taken still. (In
+        # bfloat16 swiglu has no gradient of its gradient either.)
+        if gy.dtype is torch.float16 and (torch.is_grad_enabled() or not _unwatched(gy)):
+            grads = _gated_grad_ops(gy, *ctx.saved_tensors[:3])
+            return tuple(g if n else None for g, n in zip(grads, ctx.needs_input_grad))
+        return _GatedLinear._kernels(ctx, gy)
+
+    @staticmethod
+    @_lib.once
+    def _kernels(ctx, gy):
         gy = _lib.dense(gy)
         x, wg, wu, slopes = ctx.saved_tensors
         x, wg, wu = (_lib.saved(t, gy, gy.dtype, 16) for t in (x, wg, wu))
@@ -369,24 +388,33 @@ class _GatedLinear(torch.autograd.Function):
 
 
 GATED_MAX_WIDTH = 1 << 20
+_DENSE = (torch.Tensor, nn.Parameter)
+
+
+def _ordinary(*ts) -> bool:
+    """Whether the tensors are nothing but memory that a kernel can be handed: no subclass, which may hold its
+    numbers elsewhere, and nothing that torch traces or transforms."""
+    return all(type(t) in _DENSE for t in ts) and _unwatched(*ts) and not torch.jit.is_tracing()
 
 
 def gated_linear(x: torch.Tensor, gate: nn.Linear, up: nn.Linear) -> torch.Tensor:
     """silu(gate(x)) * up(x), the input of the feed-forward block's down projection, in one kernel on
     the GPU in bfloat16 and float16: both products in fp32, their product rounded once.
     Differentiable in x and both weights; for the gradient the forward keeps the result's derivatives by
-    both products, in 20 bits. Widths that are multiples of 8, up to 2^20. Other widths, types and devices, modules with
-    a bias, hooks or a forward of their own, and torch.autocast take linear and swiglu."""
-    if isinstance(gate, fp8.Fp8Linear) or isinstance(up, fp8.Fp8Linear):
+    both products, in 20 bits. Widths that are multiples of 8, up to 2^20. Other widths, types and devices, modules
+    with a bias, hooks or a forward of their own, weights of another tensor class, torch.autocast, forward mode,
+    functional transforms and tracing take linear and swiglu. In float16 the gradients have gradients, in torch's
+    operations."""
+    if torch.compiler.is_compiling() or not (_plain(gate, nn.Linear) and _plain(up, nn.Linear)):
         return swiglu(linear(x, gate), linear(x, up))
     wg, wu = gate.weight, up.weight
     K = x.shape[-1] if x.dim() else 0
-    if not (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and wg.dtype is wu.dtype is x.dtype
+    if not (_ordinary(x, wg, wu) and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and wg.dtype is wu.dtype is x.dtype
             and wg.device == wu.device == x.device and wg.shape == wu.shape and wg.dim() == 2
             and wg.shape[1] == K and K % 8 == 0 and wg.shape[0] % 8 == 0
             and 0 < K <= GATED_MAX_WIDTH and 0 < wg.shape[0] <= GATED_MAX_WIDTH
             and x.numel() and x.numel() // K < 1 << 30 and gate.bias is None and up.bias is None
-            and _plain(gate, nn.Linear) and _plain(up, nn.Linear) and not torch.is_autocast_enabled()):
+            and not torch.is_autocast_enabled()):
         return swiglu(linear(x, gate), linear(x, up))
     x, wg, wu = (_lib.placed(_lib.dense(t), 16) for t in (x, wg, wu))
     if _lib.needs_grad(x, wg, wu):
