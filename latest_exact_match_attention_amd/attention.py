@@ -234,15 +234,14 @@ def _hard_z(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 GRAD_KERNEL_T = 1 << 20
 
 
-def _unwatched(*ts: torch.Tensor) -> bool:
-    """Whether no forward mode, dispatch mode or functional transform looks at operations on the tensors.
+def _unwatched(gy: torch.Tensor) -> bool:
+    """Whether no forward mode, dispatch mode or functional transform looks at operations on gy.
     torch has no public name for these; one that is missing or renamed counts as a yes to them."""
     try:
         ft = torch._C._functorch
-        if torch._C._len_torch_dispatch_stack() != 0 or torch.autograd.forward_ad._current_level >= 0:
-            return False
-        return not any(ft.is_functorch_wrapped_tensor(t) or ft.is_legacy_batchedtensor(t) or t._is_zerotensor()
-                       for t in ts)
+        return (torch._C._len_torch_dispatch_stack() == 0
+                and not ft.is_functorch_wrapped_tensor(gy) and not ft.is_legacy_batchedtensor(gy)
+                and torch.autograd.forward_ad._current_level < 0 and not gy._is_zerotensor())
     except AttributeError:
         return False
 

@@ -389,12 +389,25 @@ class _GatedLinear(torch.autograd.Function):
 
 GATED_MAX_WIDTH = 1 << 20
 _DENSE = (torch.Tensor, nn.Parameter)
+_C, _FORWARD_AD, _compiling = torch._C, torch.autograd.forward_ad, torch.compiler.is_compiling
 
 
-def _ordinary(*ts) -> bool:
+def _parameter(mod: nn.Module, name: str):
+    """mod.name, without the module's own lookup (0.4 us) where it is a parameter."""
+    ps = mod._parameters
+    return ps[name] if name in ps else getattr(mod, name)
+
+
+def _ordinary(x, wg, wu) -> bool:
     """Whether the tensors are nothing but memory that a kernel can be handed: no subclass, which may hold its
-    numbers elsewhere, and nothing that torch traces or transforms."""
-    return all(type(t) in _DENSE for t in ts) and _unwatched(*ts) and not torch.jit.is_tracing()
+    numbers elsewhere, and nothing that torch traces or transforms. torch has no public names for most of
+    these; one that is missing counts as a yes to them."""
+    try:
+        return (type(x) in _DENSE and type(wg) in _DENSE and type(wu) in _DENSE
+                and not _C._are_functorch_transforms_active() and _C._len_torch_dispatch_stack() == 0
+                and _FORWARD_AD._current_level < 0 and not _C._is_tracing())
+    except AttributeError:
+        return False
 
 
 def gated_linear(x: torch.Tensor, gate: nn.Linear, up: nn.Linear) -> torch.Tensor:
@@ -405,15 +418,16 @@ def gated_linear(x: torch.Tensor, gate: nn.Linear, up: nn.Linear) -> torch.Tenso
     with a bias, hooks or a forward of their own, weights of another tensor class, torch.autocast, forward mode,
     functional transforms and tracing take linear and swiglu. In float16 the gradients have gradients, in torch's
     operations."""
-    if torch.compiler.is_compiling() or not (_plain(gate, nn.Linear) and _plain(up, nn.Linear)):
+    if _compiling() or not (_plain(gate, nn.Linear) and _plain(up, nn.Linear)):
         return swiglu(linear(x, gate), linear(x, up))
-    wg, wu = gate.weight, up.weight
+    wg, wu = _parameter(gate, "weight"), _parameter(up, "weight")
     K = x.shape[-1] if x.dim() else 0
     if not (_ordinary(x, wg, wu) and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and wg.dtype is wu.dtype is x.dtype
             and wg.device == wu.device == x.device and wg.shape == wu.shape and wg.dim() == 2
             and wg.shape[1] == K and K % 8 == 0 and wg.shape[0] % 8 == 0
             and 0 < K <= GATED_MAX_WIDTH and 0 < wg.shape[0] <= GATED_MAX_WIDTH
-            and x.numel() and x.numel() // K < 1 << 30 and gate.bias is None and up.bias is None
+            and x.numel() and x.numel() // K < 1 << 30
+            and _parameter(gate, "bias") is None and _parameter(up, "bias") is None
             and not torch.is_autocast_enabled()):
         return swiglu(linear(x, gate), linear(x, up))
     x, wg, wu = (_lib.placed(_lib.dense(t), 16) for t in (x, wg, wu))
@@ -726,7 +740,8 @@ class SwiGLU(nn.Module):
 
     def _fp8(self) -> bool:
         """Whether one of the weights is held in 8 bits."""
-        return any(isinstance(lin, fp8.Fp8Linear) for lin in (self.gate, self.up, self.down))
+        kind = fp8.Fp8Linear
+        return isinstance(self.gate, kind) or isinstance(self.up, kind) or isinstance(self.down, kind)
 
     def forward_normed(self, x, d, norm: nn.RMSNorm):
         """x + d + self(norm(x + d)), Block.forward's MLP half, on decode shapes: the norm runs
