@@ -8,8 +8,9 @@
 // each keeps a head of that order. The token is the first in vocabulary order whose running sum of
 // kept w exceeds u times their sum. The log-probability is (z_i - max) / T - log sum of all w.
 //
-// One workgroup of 1024 threads a row. A row of up to 128 KB is held in LDS and read once from memory; a
-// longer one is read again in each pass, from the caches. A single CU's arithmetic is what bounds a row
+// One workgroup of 1024 threads a row. A row of up to 128 KB is held in LDS and read once from memory, one of up
+// to 256 KB in registers for the passes that every row takes; otherwise it is read again in each pass, from
+// the caches. A single CU's arithmetic is what bounds a row
 // (an instruction for each of 50,304 logits takes 0.33 us), so the passes over it are few and short:
 //   1  the maximum, of the row and of each thread's part of it;
 //   2  the sum of all w, and a list of those tokens that can be kept: not below min-p's border, nor below
@@ -485,7 +486,7 @@ __device__ __forceinline__ float setting(const Setting& s, int64_t r) {
   return s.each ? static_cast<const float*>(s.each)[r] : s.one;
 }
 
-// Choices, each with the times of both sides for 64 rows of 50,304 bf16 logits.
+// Choices, each with the times of both sides for 64 rows of 50,304 bf16 logits (measured at that size alone).
 // Candidates that are ranked by counting: 54 of them (top-k 50, one row) 15.1 us, sorted 20.3; about 250 of them
 // take the same both ways.
 constexpr int kFew = 256;

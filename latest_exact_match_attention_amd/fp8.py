@@ -1,5 +1,5 @@
-"""Products in 8-bit floating point for serving: half of bf16's weight bytes in a decode step, and the
-matrix cores' 8-bit rate in a prefill.
+"""Products in 8-bit floating point for serving: half of bf16's weight bytes, and the matrix cores' 8-bit
+rate in a prefill.
 
     quantize(x, block_rows)          e4m3 values with a power-of-two scale for each block of 128
     matmul(a, w)                     a . w^T of quantized operands
@@ -276,7 +276,10 @@ def quantize_feed_forward(model: nn.Module, head: bool = False) -> nn.Module:
     """Holds the feed-forward weights of a Transformer's blocks (and with `head` the head's) in 8 bits, in
     place, for serving; returns the model. The query and key projections keep their type: their
     outputs' signs are the codes that are matched exactly, and the value and output projections are
-    small beside the feed-forward ones. A model's state_dict then loads into one that was held so, too."""
+    small beside the feed-forward ones. A model's state_dict then loads into one that was held so, too.
+
+    It pays in prefills (3 to 20% in a bf16 model of 24 layers of 1536) and in decode steps of 16 streams
+    (1%) and more (32: 10%); steps of one to four streams take 18 to 25% longer."""
     for block in model.blocks:
         for name in ("gate", "up", "down"):
             lin = getattr(block.mlp, name)
