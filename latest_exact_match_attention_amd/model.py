@@ -418,11 +418,12 @@ def gated_linear(x: torch.Tensor, gate: nn.Linear, up: nn.Linear) -> torch.Tenso
     with a bias, hooks or a forward of their own, weights of another tensor class, torch.autocast, forward mode,
     functional transforms and tracing take linear and swiglu. In float16 the gradients have gradients, in torch's
     operations."""
-    if _compiling() or not (_plain(gate, nn.Linear) and _plain(up, nn.Linear)):
+    if not (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and not _compiling()
+            and _plain(gate, nn.Linear) and _plain(up, nn.Linear)):
         return swiglu(linear(x, gate), linear(x, up))
     wg, wu = _parameter(gate, "weight"), _parameter(up, "weight")
     K = x.shape[-1] if x.dim() else 0
-    if not (_ordinary(x, wg, wu) and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and wg.dtype is wu.dtype is x.dtype
+    if not (_ordinary(x, wg, wu) and wg.dtype is wu.dtype is x.dtype
             and wg.device == wu.device == x.device and wg.shape == wu.shape and wg.dim() == 2
             and wg.shape[1] == K and K % 8 == 0 and wg.shape[0] % 8 == 0
             and 0 < K <= GATED_MAX_WIDTH and 0 < wg.shape[0] <= GATED_MAX_WIDTH
