@@ -937,9 +937,10 @@ class Transformer(nn.Module):
             forward(next, cache=c)                    extending c
 
         With a cache, queries match keys from before this call too, so a sequence can be fed
-        in pieces: every piece's numbers are rounded alike, though a 16-bit sum's last bit can
-        depend on how many rows a call has (another order of its terms in fp32). In bf16 on the GPU nothing of a call
-        with a cache has a gradient, its logits neither. Tokens must lie in [0, vocab_size); on the
+        in pieces; any chunking gives the one-shot result but for last bits, which can depend on
+        how many rows a call has: fp32 sums take another order, and in bf16 on the GPU a block of
+        more than 32 rows adds its residual before the down product is rounded, one of fewer
+        after. There nothing of a call with a cache has a gradient, its logits neither. Tokens must lie in [0, vocab_size); on the
         GPU they are not checked.
         """
         if cache is not None and not (self.lema_layers()

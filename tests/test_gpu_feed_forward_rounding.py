@@ -1,5 +1,5 @@
-"""A token's feed-forward block gives the same numbers in a decode step, a chunk and a prompt: both products
-in fp32, silu(g) * u rounded once, however many rows a call has."""
+"""A token's gated product is the same in a decode step, a chunk and a prompt: both products in fp32,
+silu(g) * u rounded once, however many rows a call has."""
 import pytest
 import torch
 
